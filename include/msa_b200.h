@@ -441,6 +441,35 @@ int msa_index_kl_dik(const void* index_q, int dtype, const int32_t* cu_seqlens, 
                      int32_t block_size, int32_t total_blocks, const void* g_pt, int pt_f64,
                      void* d_index_k_acc, void* workspace, size_t workspace_bytes, void* stream);
 
+/* ---------------------------------------------------------------- query/key norm and rotation
+ * The step between a layer's projections and the operators above (the reference takes
+ * normalised, rotated heads as given). Every head row x of q and k (head_dim D <= 512):
+ *   y = R(p) (w * x * r),  r = (mean(x^2) + eps)^(-1/2)
+ * with R(p) rotating the pairs of the first rotary_dim elements, (i, i + rotary_dim/2) or, with
+ * `interleaved`, (2i, 2i + 1), by row p of rope_table [table_rows][rotary_dim] (float32: cosines,
+ * then sines; rotary_dim even, 0 rotates nothing). p is positions[t] or, with positions NULL,
+ * t's offset in its sequence of cu_seqlens; a row whose p lies outside the table is NaN. q and k
+ * have the given token and head strides (elements; head rows dense), outputs are dense.
+ * Weights have the tensors' dtype or float32. The backward writes any of dq, dk (dense), dq_weight
+ * and dk_weight (NULL: not wanted; fixed-order sums, no atomics).
+ * workspace: msa_qk_norm_rope_bwd_workspace_size() bytes, used with a weight gradient only. */
+int msa_qk_norm_rope_fwd(const void* q, const void* k, int dtype, const void* q_weight, const void* k_weight,
+                         int weight_dtype, const float* rope_table, int64_t table_rows, int32_t rotary_dim,
+                         int interleaved, const int32_t* positions, const int32_t* cu_seqlens, int32_t nseq,
+                         int64_t total_tokens, int32_t q_heads, int32_t k_heads, int32_t head_dim,
+                         int64_t q_token_stride, int64_t q_head_stride, int64_t k_token_stride,
+                         int64_t k_head_stride, double eps, void* q_out, void* k_out, void* stream);
+size_t msa_qk_norm_rope_bwd_workspace_size(int32_t head_dim);
+int msa_qk_norm_rope_bwd(const void* q, const void* k, const void* grad_q, const void* grad_k, int dtype,
+                         const void* q_weight, const void* k_weight, int weight_dtype, const float* rope_table,
+                         int64_t table_rows, int32_t rotary_dim, int interleaved, const int32_t* positions,
+                         const int32_t* cu_seqlens, int32_t nseq, int64_t total_tokens, int32_t q_heads,
+                         int32_t k_heads, int32_t head_dim, int64_t q_token_stride, int64_t q_head_stride,
+                         int64_t k_token_stride, int64_t k_head_stride, int64_t gq_token_stride,
+                         int64_t gq_head_stride, int64_t gk_token_stride, int64_t gk_head_stride, double eps,
+                         void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace,
+                         size_t workspace_bytes, void* stream);
+
 /* ---------------------------------------------------------------- diagnostics
  * Self-test of the tensor-core building blocks (no counterpart in the
  * reference): one 128 x nw tile per CTA of C = A B. layout bit 0: B stored

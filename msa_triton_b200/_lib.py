@@ -89,6 +89,13 @@ _SIGNATURES = {
     "msa_index_kl_dik_workspace_size": ([c_int64, c_int32, c_int32, c_int], c_size_t),
     "msa_index_kl_dik": ([_P, c_int, _P, _P, _P, _P, _P, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
                           c_int32, _P, c_int, _P, _P, c_size_t, _P], c_int),
+    "msa_qk_norm_rope_fwd": ([_P, _P, c_int, _P, _P, c_int, _P, c_int64, c_int32, c_int, _P, _P, c_int32, c_int64,
+                              c_int32, c_int32, c_int32, c_int64, c_int64, c_int64, c_int64, c_double, _P, _P, _P],
+                             c_int),
+    "msa_qk_norm_rope_bwd_workspace_size": ([c_int32], c_size_t),
+    "msa_qk_norm_rope_bwd": ([_P, _P, _P, _P, c_int, _P, _P, c_int, _P, c_int64, c_int32, c_int, _P, _P, c_int32,
+                              c_int64, c_int32, c_int32, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64,
+                              c_int64, c_int64, c_int64, c_double, _P, _P, _P, _P, _P, c_size_t, _P], c_int),
     "msa_attn_bwd_atomic": ([_P, _P, _P, _P, c_int, _P, _P, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
                              c_int32, c_double, _P, _P, _P, _P, _P, _P, _P], c_int),
 }

@@ -23,6 +23,8 @@ differentiable):
 * ``msa_b200::sparse_attention(q, k, v, indices, cu, bounds, block_size, scale)
   -> (out, lse, lse64, row_ptr, query_indices, slot_indices, cu_block_lens)``;
   ``msa_b200::sparse_attention_backward``.
+* ``msa_b200::qk_norm_rope(q, k, q_weight, k_weight, rope_table, positions, cu, eps, interleaved)
+  -> (q_out, k_out)``; ``msa_b200::qk_norm_rope_backward``.
 """
 
 from __future__ import annotations
@@ -32,6 +34,7 @@ from torch import Tensor
 
 from . import _dispatch
 from . import index_score as _score
+from . import qk_norm_rope as _rope
 from . import sparse_attention as _attn
 from . import topk as _topk
 from .k2q import K2QCSR
@@ -201,3 +204,52 @@ def sparse_attention(q, k, v, indices, cu_seqlens, bounds, block_size, scale) ->
     """(out, lse) of ``msa_b200::sparse_attention`` (arguments already validated)."""
     res = torch.ops.msa_b200.sparse_attention(q, k, v, indices, cu_seqlens, list(bounds), block_size, scale)
     return res[0], res[1]
+
+
+# ----------------------------------------------------------------------------- query/key norm and rotation
+@torch.library.custom_op("msa_b200::qk_norm_rope", mutates_args=(), device_types="cuda")
+def _qk_norm_rope_op(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, rope_table: Tensor,
+                     positions: Tensor | None, cu_seqlens: Tensor | None, eps: float,
+                     interleaved: bool) -> tuple[Tensor, Tensor]:
+    return _rope.norm_rope_forward(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, interleaved)
+
+
+@_qk_norm_rope_op.register_fake
+def _(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, interleaved):
+    return q.new_empty(q.shape), k.new_empty(k.shape)
+
+
+@torch.library.custom_op("msa_b200::qk_norm_rope_backward", mutates_args=(), device_types="cuda")
+def _qk_norm_rope_backward_op(q: Tensor, k: Tensor, q_weight: Tensor, k_weight: Tensor, rope_table: Tensor,
+                              positions: Tensor | None, cu_seqlens: Tensor | None, eps: float, interleaved: bool,
+                              grad_q: Tensor, grad_k: Tensor,
+                              need: list[bool]) -> tuple[Tensor, Tensor, Tensor, Tensor]:
+    grads = _rope.norm_rope_backward(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, interleaved,
+                                     grad_q, grad_k, need)
+    return tuple(_empty_like_or(g, x) for g, x in zip(grads, (q, k, q_weight, k_weight)))
+
+
+@_qk_norm_rope_backward_op.register_fake
+def _(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, interleaved, grad_q, grad_k, need):
+    return tuple(x.new_empty(x.shape if n else (0,)) for x, n in zip((q, k, q_weight, k_weight), need))
+
+
+def _qk_norm_rope_setup(ctx, inputs, output):
+    *tensors, eps, interleaved = inputs
+    ctx.save_for_backward(*tensors)
+    ctx.meta = (eps, interleaved)
+
+
+def _qk_norm_rope_bwd(ctx, grad_q, grad_k):
+    need = list(ctx.needs_input_grad[:4])
+    grads = torch.ops.msa_b200.qk_norm_rope_backward(*ctx.saved_tensors, *ctx.meta, grad_q, grad_k, need)
+    return (*(_none_if_empty(g, n) for g, n in zip(grads, need)), None, None, None, None, None)
+
+
+_qk_norm_rope_op.register_autograd(_qk_norm_rope_bwd, setup_context=_qk_norm_rope_setup)
+
+
+def qk_norm_rope(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, interleaved) -> tuple[Tensor, Tensor]:
+    """(q_out, k_out) of ``msa_b200::qk_norm_rope`` (arguments already validated)."""
+    return torch.ops.msa_b200.qk_norm_rope(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, float(eps),
+                                           bool(interleaved))
