@@ -42,7 +42,7 @@ enum {
   MSA_ERR_TIMEOUT = 4,
 };
 
-enum { MSA_F32 = 0, MSA_F16 = 1, MSA_BF16 = 2 };
+enum { MSA_F32 = 0, MSA_F16 = 1, MSA_BF16 = 2, MSA_E4M3 = 3 /* 8-bit caches only */ };
 
 /* Library version string and the calling thread's last error message. */
 const char* msa_version(void);
@@ -469,6 +469,27 @@ int msa_qk_norm_rope_bwd(const void* q, const void* k, const void* grad_q, const
                          int64_t gq_head_stride, int64_t gk_token_stride, int64_t gk_head_stride, double eps,
                          void* dq, void* dk, void* dq_weight, void* dk_weight, void* workspace,
                          size_t workspace_bytes, void* stream);
+
+/* ---------------------------------------------------------------- paged cache append
+ * New keys and values of `batch` requests into their pages, the keys rotated on the way (as
+ * msa_qk_norm_rope_fwd rotates; rotary_dim 0: stored as they are). k and v: [total_tokens][heads][D]
+ * with the given strides; request b's rows are cu_seqlens[b] .. cu_seqlens[b+1]-1, or row b with
+ * cu_seqlens NULL, and take the last positions of its seq_lens[b] tokens. v NULL: keys only. Caches
+ * [num_pages][page_size][heads][D] with the given strides (dense head rows), of the inputs' dtype or
+ * MSA_E4M3 with float32 scales [num_pages][heads]: a code c stands for c * scale. The append keeps
+ * scales at powers of two, the smallest with every new value at most 448 * scale; a page that held
+ * earlier rows keeps a larger scale or moves them to the new one. Values that are not finite become
+ * NaN codes and do not count for the scale. A key whose position lies outside the table is NaN. Rows
+ * behind the last request, positions below 0 and pages outside the block table's max_pages or the
+ * cache are skipped. A page receives tokens of one request only. */
+int msa_cache_append(const void* k, const void* v, int dtype, int64_t k_token_stride, int64_t k_head_stride,
+                     int64_t v_token_stride, int64_t v_head_stride, const float* rope_table, int64_t table_rows,
+                     int32_t rotary_dim, int interleaved, const int32_t* cu_seqlens, const int32_t* block_table,
+                     const int32_t* seq_lens, int32_t batch, int64_t total_tokens, int32_t heads, int32_t head_dim,
+                     int32_t page_size, int32_t max_pages, int64_t num_pages, void* k_cache, void* v_cache,
+                     int cache_dtype, int64_t k_page_stride, int64_t k_slot_stride, int64_t k_cache_head_stride,
+                     int64_t v_page_stride, int64_t v_slot_stride, int64_t v_cache_head_stride, float* k_scale,
+                     float* v_scale, void* stream);
 
 /* ---------------------------------------------------------------- diagnostics
  * Self-test of the tensor-core building blocks (no counterpart in the

@@ -17,6 +17,7 @@ import torch
 LIB_PATH = Path(__file__).resolve().parent / "libmsa_b200.so"
 
 DTYPE_CODE = {torch.float32: 0, torch.float16: 1, torch.bfloat16: 2}
+E4M3_CODE = 3  # 8-bit caches
 
 _P = c_void_p
 _SIGNATURES = {
@@ -96,6 +97,9 @@ _SIGNATURES = {
     "msa_qk_norm_rope_bwd": ([_P, _P, _P, _P, c_int, _P, _P, c_int, _P, c_int64, c_int32, c_int, _P, _P, c_int32,
                               c_int64, c_int32, c_int32, c_int32, c_int64, c_int64, c_int64, c_int64, c_int64,
                               c_int64, c_int64, c_int64, c_double, _P, _P, _P, _P, _P, c_size_t, _P], c_int),
+    "msa_cache_append": ([_P, _P, c_int, c_int64, c_int64, c_int64, c_int64, _P, c_int64, c_int32, c_int, _P, _P, _P,
+                          c_int32, c_int64, c_int32, c_int32, c_int32, c_int32, c_int64, _P, _P, c_int, c_int64,
+                          c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P], c_int),
     "msa_attn_bwd_atomic": ([_P, _P, _P, _P, c_int, _P, _P, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
                              c_int32, c_double, _P, _P, _P, _P, _P, _P, _P], c_int),
 }

@@ -1,0 +1,134 @@
+"""New keys and values into a paged KV cache, in the inputs' type or in 8 bits.
+
+The caches are those the decode operators read (``decode.py``): ``[P, S, G, D]``,
+P physical pages of S tokens, addressed through a block table. One call per cache
+stores the newest tokens of every request, rotating the keys on the way:
+
+    m3_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, rope_table=table)      # one token per request
+    m3_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, cu_seqlens=cu)         # packed chunks
+    m3_cache_append(index_k, None, index_k_cache, None, block_table, seq_lens)            # the indexer's keys
+
+8-bit caches are ``torch.float8_e4m3fn`` with float32 scales ``[P, G]``, one per page and
+head: a code ``c`` stands for ``c * scale``. The append chooses powers of two, the smallest
+with every value at most ``448 * scale`` (e4m3 is a floating format, so that costs no
+precision); a page that already holds tokens keeps its scale unless the new ones need a
+larger one, and then its earlier codes move to it, exactly as long as they stay normal
+numbers. ``m3_sparse_decode`` reads such a cache with ``k_scale=`` / ``v_scale=``.
+Inference only (no autograd). CUDA tensors only.
+"""
+
+from __future__ import annotations
+
+import torch
+
+from . import _lib
+from ._lib import DTYPE_CODE, E4M3_CODE, call, ptr, stream_of
+from .decode import _check_paged
+from .qk_norm_rope import check_table, dense_rows
+
+CACHE_8BIT = torch.float8_e4m3fn
+
+
+def check_scale(name, scale, cache):
+    """The scales of an 8-bit cache ``[P, S, G, D]``: float32 ``[P, G]``, dense."""
+    if scale is None or scale.shape != (cache.shape[0], cache.shape[2]) or scale.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32 [P,G] for an 8-bit cache")
+    if scale.device != cache.device:
+        raise ValueError("All inputs must reside on the same device.")
+    if not scale.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
+def _check_cache(name, x, cache, scale, device):
+    if cache.ndim != 4 or cache.shape[2:] != x.shape[1:]:
+        raise ValueError(f"expected {name}_cache[P,S,G,D] with {name}'s G and D")
+    if cache.device != device:
+        raise ValueError("All inputs must reside on the same device.")
+    if cache.shape[1] < 1:
+        raise ValueError("pages must hold at least one token")
+    if cache.dtype == CACHE_8BIT:
+        check_scale(f"{name}_scale", scale, cache)
+    elif cache.dtype != x.dtype:
+        raise TypeError("a cache must have the inputs' dtype or float8_e4m3fn")
+    elif scale is not None:
+        raise ValueError(f"{name}_scale belongs to an 8-bit cache")
+    # written in place: head rows must be dense, and no two elements may share memory
+    if cache.shape[3] > 1 and cache.stride(3) != 1:
+        raise ValueError(f"{name}_cache must have dense head rows")
+    span = 1
+    for stride, size in sorted((cache.stride(i), cache.shape[i]) for i in range(4) if cache.shape[i] > 1):
+        if stride < span:
+            raise ValueError(f"{name}_cache must not overlap itself")
+        span = stride * size
+
+
+@torch.no_grad()
+def m3_cache_append(
+    k: torch.Tensor,
+    v: torch.Tensor | None,
+    k_cache: torch.Tensor,
+    v_cache: torch.Tensor | None,
+    block_table: torch.Tensor,
+    seq_lens: torch.Tensor,
+    *,
+    cu_seqlens: torch.Tensor | None = None,
+    rope_table: torch.Tensor | None = None,
+    interleaved: bool = False,
+    k_scale: torch.Tensor | None = None,
+    v_scale: torch.Tensor | None = None,
+) -> None:
+    """Store the newest tokens ``k[T,G,D]`` (and ``v``, or None) of B requests in their pages.
+
+    ``seq_lens[B]`` (int32) counts each request's tokens with the new ones; request b's new
+    rows are ``cu_seqlens[b] .. cu_seqlens[b+1] - 1`` (int32 ``[B + 1]``, on the device, not read
+    by the host), or row b without ``cu_seqlens`` (``T = B``), and take its last positions.
+    ``rope_table`` rotates the keys as ``m3_qk_norm_rope`` does; without it they are stored as
+    they are. Caches ``[P,S,G,D]`` are written in place; ``k_scale`` / ``v_scale`` come with 8-bit
+    ones. Skipped, with nothing written: rows behind ``cu_seqlens[B]``, requests of length 0 (a
+    padded batch), pages past the block table's width or outside the cache. A page that receives
+    tokens must belong to one request.
+    """
+    if k.ndim != 3 or (v is not None and v.shape != k.shape):
+        raise ValueError("expected k[T,G,D] and a matching v")
+    if (v is None) != (v_cache is None):
+        raise ValueError("v and v_cache go together")
+    if k.dtype not in (torch.bfloat16, torch.float16, torch.float32) or (v is not None and v.dtype != k.dtype):
+        raise TypeError("k/v must share a BF16, FP16, or FP32 dtype.")
+    total, heads, dim = k.shape
+    if heads <= 0 or dim <= 0:
+        raise ValueError("expected at least one head and a positive head dimension")
+    if v is not None and v.device != k.device:
+        raise ValueError("All inputs must reside on the same device.")
+    _check_cache("k", k, k_cache, k_scale, k.device)
+    if v is not None:
+        _check_cache("v", v, v_cache, v_scale, k.device)
+        if v_cache.shape[:2] != k_cache.shape[:2] or v_cache.dtype != k_cache.dtype:
+            raise ValueError("k_cache and v_cache must share their pages and dtype")
+    elif v_scale is not None:
+        raise ValueError("v_scale belongs to an 8-bit cache")
+    batch = seq_lens.shape[0] if seq_lens.ndim == 1 else -1
+    _check_paged(block_table, seq_lens, batch, k.device)
+    if cu_seqlens is None:
+        if total != batch:
+            raise ValueError("without cu_seqlens, k holds one token per request")
+    elif cu_seqlens.shape != (batch + 1,) or cu_seqlens.dtype != torch.int32:
+        raise ValueError("cu_seqlens must be int32 [B + 1]")
+    elif cu_seqlens.device != k.device:
+        raise ValueError("All inputs must reside on the same device.")
+    if rope_table is not None:
+        check_table(rope_table, dim, k.device)
+    _lib.require_cuda(k)
+    kd, vd = dense_rows(k), None if v is None else dense_rows(v)
+    table = None if rope_table is None else rope_table.contiguous()
+    rows, rotary = (0, 0) if table is None else table.shape
+    # held by name until the launch: a temporary's memory would be handed to the next copy
+    cu = None if cu_seqlens is None else cu_seqlens.contiguous()
+    pages, lens = block_table.contiguous(), seq_lens.contiguous()
+    v_strides = (0, 0) if v is None else (vd.stride(0), vd.stride(1))
+    v_cache_strides = (0, 0, 0) if v is None else v_cache.stride()[:3]
+    with torch.cuda.device(k.device):
+        call("msa_cache_append", ptr(kd), ptr(vd), DTYPE_CODE[k.dtype], kd.stride(0), kd.stride(1), *v_strides,
+             ptr(table), rows, rotary, int(interleaved), ptr(cu), ptr(pages), ptr(lens), batch, total,
+             heads, dim, k_cache.shape[1], block_table.shape[1], k_cache.shape[0], ptr(k_cache), ptr(v_cache),
+             E4M3_CODE if k_cache.dtype == CACHE_8BIT else DTYPE_CODE[k_cache.dtype], *k_cache.stride()[:3],
+             *v_cache_strides, ptr(k_scale), ptr(v_scale), stream_of(k))
