@@ -491,6 +491,19 @@ int msa_cache_append(const void* k, const void* v, int dtype, int64_t k_token_st
                      int64_t v_page_stride, int64_t v_slot_stride, int64_t v_cache_head_stride, float* k_scale,
                      float* v_scale, void* stream);
 
+/* ---------------------------------------------------------------- decode over an 8-bit cache
+ * msa_decode_attn over e4m3 caches [num_pages][page_size][groups][D] (strides in bytes, dense head
+ * rows, D <= 256) with float32 scales [num_pages][groups], as msa_cache_append fills them; any number of
+ * query heads per group. q and out [batch][q_heads][D] dense, lse [batch][q_heads]. Keys on pages outside
+ * the block table's max_pages or the cache are not attended. One launch, no workspace. */
+int msa_decode_attn_e4m3(const void* q, int dtype, const void* k_cache, const void* v_cache, int64_t k_page_stride,
+                         int64_t k_slot_stride, int64_t k_head_stride, int64_t v_page_stride, int64_t v_slot_stride,
+                         int64_t v_head_stride, const float* k_scale, const float* v_scale,
+                         const int32_t* block_table, const int32_t* seq_lens, const int32_t* indices, int32_t batch,
+                         int32_t q_heads, int32_t groups, int32_t head_dim, int32_t page_size, int32_t max_pages,
+                         int64_t num_pages, int32_t topk_blocks, int32_t block_size, double scale, void* out,
+                         float* lse, void* stream);
+
 /* ---------------------------------------------------------------- diagnostics
  * Self-test of the tensor-core building blocks (no counterpart in the
  * reference): one 128 x nw tile per CTA of C = A B. layout bit 0: B stored

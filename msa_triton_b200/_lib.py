@@ -100,6 +100,9 @@ _SIGNATURES = {
     "msa_cache_append": ([_P, _P, c_int, c_int64, c_int64, c_int64, c_int64, _P, c_int64, c_int32, c_int, _P, _P, _P,
                           c_int32, c_int64, c_int32, c_int32, c_int32, c_int32, c_int64, _P, _P, c_int, c_int64,
                           c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P], c_int),
+    "msa_decode_attn_e4m3": ([_P, c_int, _P, _P, c_int64, c_int64, c_int64, c_int64, c_int64, c_int64, _P, _P, _P, _P,
+                              _P, c_int32, c_int32, c_int32, c_int32, c_int32, c_int32, c_int64, c_int32, c_int32,
+                              c_double, _P, _P, _P], c_int),
     "msa_attn_bwd_atomic": ([_P, _P, _P, _P, c_int, _P, _P, c_int32, c_int64, c_int32, c_int32, c_int32, c_int32,
                              c_int32, c_double, _P, _P, _P, _P, _P, _P, _P], c_int),
 }

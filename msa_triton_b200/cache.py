@@ -23,21 +23,8 @@ import torch
 
 from . import _lib
 from ._lib import DTYPE_CODE, E4M3_CODE, call, ptr, stream_of
-from .decode import _check_paged
+from .decode import CACHE_8BIT, _check_paged, check_scale
 from .qk_norm_rope import check_table, dense_rows
-
-CACHE_8BIT = torch.float8_e4m3fn
-
-
-def check_scale(name, scale, cache):
-    """The scales of an 8-bit cache ``[P, S, G, D]``: float32 ``[P, G]``, dense."""
-    if scale is None or scale.shape != (cache.shape[0], cache.shape[2]) or scale.dtype != torch.float32:
-        raise ValueError(f"{name} must be float32 [P,G] for an 8-bit cache")
-    if scale.device != cache.device:
-        raise ValueError("All inputs must reside on the same device.")
-    if not scale.is_contiguous():
-        raise ValueError(f"{name} must be contiguous")
-
 
 def _check_cache(name, x, cache, scale, device):
     if cache.ndim != 4 or cache.shape[2:] != x.shape[1:]:

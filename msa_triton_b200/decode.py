@@ -10,6 +10,8 @@ contributing its newest token (position ``seq_lens[b] - 1``) as the query:
     indices = m3_topk_decode(scores, seq_lens, topk_blocks=16, local_blocks=1)
     out     = m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices)
 
+``m3_cache_append`` fills the caches; ``m3_sparse_decode`` also reads its 8-bit ones.
+
 Layouts: ``index_q[B,G,Di]``, ``q[B,Hq,D]``; caches ``index_k_cache[P,S,1,Di]``,
 ``k_cache/v_cache[P,S,G,D]`` (P physical pages of S tokens); ``block_table[B, max_pages]``
 int32 physical page of each logical page; ``seq_lens[B]`` int32 keys per request
@@ -86,19 +88,42 @@ def m3_topk_decode(scores, seq_lens, *, block_size=128, topk_blocks=16, local_bl
     return out
 
 
+CACHE_8BIT = torch.float8_e4m3fn
+
+
+def check_scale(name, scale, cache):
+    """The scales of an 8-bit cache ``[P, S, G, D]``: float32 ``[P, G]``, dense."""
+    if scale is None or scale.shape != (cache.shape[0], cache.shape[2]) or scale.dtype != torch.float32:
+        raise ValueError(f"{name} must be float32 [P,G] for an 8-bit cache")
+    if scale.device != cache.device:
+        raise ValueError("All inputs must reside on the same device.")
+    if not scale.is_contiguous():
+        raise ValueError(f"{name} must be contiguous")
+
+
 @torch.no_grad()
 def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, block_size=128, scale=None,
-                     return_lse=False):
-    """Sparse attention of each request's new token over its selected cached blocks."""
+                     return_lse=False, k_scale=None, v_scale=None):
+    """Sparse attention of each request's new token over its selected cached blocks.
+
+    With 8-bit caches (``torch.float8_e4m3fn``), ``k_scale`` / ``v_scale`` (float32 ``[P,G]``) hold
+    what ``m3_cache_append`` keeps: a code of page p and head g stands for ``code * scale[p, g]``.
+    The caches may then have any strides with dense head rows."""
     if q.ndim != 3 or k_cache.ndim != 4 or v_cache.shape != k_cache.shape:
         raise ValueError("expected q[B,Hq,D] and k_cache/v_cache[P,S,G,D]")
     batch, hq, dim = q.shape
     groups = k_cache.shape[2]
     if k_cache.shape[3] != dim or hq % groups:
         raise ValueError("Hq must be a multiple of G and D must match the cache")
-    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32) or k_cache.dtype != q.dtype or \
-            v_cache.dtype != q.dtype:
+    quantised = k_cache.dtype == CACHE_8BIT
+    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32) or v_cache.dtype != k_cache.dtype or \
+            not (quantised or k_cache.dtype == q.dtype):
         raise TypeError("q/k/v must share a BF16, FP16, or FP32 dtype.")
+    if quantised:
+        check_scale("k_scale", k_scale, k_cache)
+        check_scale("v_scale", v_scale, v_cache)
+    elif k_scale is not None or v_scale is not None:
+        raise ValueError("k_scale and v_scale belong to an 8-bit cache")
     if indices.ndim != 3 or indices.shape[:2] != (batch, groups) or indices.dtype != torch.int32:
         raise ValueError("indices must be int32 [B,G,K].")
     if not isinstance(block_size, int) or block_size <= 0:
@@ -107,7 +132,12 @@ def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, blo
     if not math.isfinite(effective):
         raise ValueError("scale must be finite.")
     _check_paged(block_table, seq_lens, batch, q.device)
+    if quantised and any(x.device != q.device for x in (k_cache, v_cache, indices)):
+        raise ValueError("All inputs must reside on the same device.")
     _lib.require_cuda(q)
+    if quantised:
+        return _sparse_decode8(q, k_cache, v_cache, block_table, seq_lens, indices, block_size, effective, return_lse,
+                               k_scale, v_scale)
     out = torch.empty_like(q)
     lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device)
     if batch:
@@ -120,4 +150,20 @@ def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, blo
             call("msa_decode_attn", ptr(qc), ptr(kc), ptr(vc), DTYPE_CODE[q.dtype], ptr(block_table.contiguous()),
                  ptr(seq_lens), ptr(indices.contiguous()), batch, hq, groups, dim, kc.shape[1], block_table.shape[1],
                  topk, block_size, effective, ptr(out), ptr(lse), ptr(ws), ws_bytes, stream_of(q))
+    return (out, lse) if return_lse else out
+
+
+def _sparse_decode8(q, k_cache, v_cache, block_table, seq_lens, indices, block_size, scale, return_lse, k_scale,
+                    v_scale):
+    batch, hq, dim = q.shape
+    out = torch.empty((batch, hq, dim), dtype=q.dtype, device=q.device)
+    lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device)
+    if batch and dim:
+        dense = [x if x.shape[3] == 1 or x.stride(3) == 1 else x.contiguous() for x in (k_cache, v_cache)]
+        qc, table, lens, ids = q.contiguous(), block_table.contiguous(), seq_lens.contiguous(), indices.contiguous()
+        with torch.cuda.device(q.device):
+            call("msa_decode_attn_e4m3", ptr(qc), DTYPE_CODE[q.dtype], ptr(dense[0]), ptr(dense[1]),
+                 *dense[0].stride()[:3], *dense[1].stride()[:3], ptr(k_scale), ptr(v_scale), ptr(table), ptr(lens),
+                 ptr(ids), batch, hq, k_cache.shape[2], dim, k_cache.shape[1], table.shape[1], k_cache.shape[0],
+                 ids.shape[2], block_size, scale, ptr(out), ptr(lse), stream_of(q))
     return (out, lse) if return_lse else out

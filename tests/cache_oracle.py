@@ -74,21 +74,27 @@ def append(k, v, k_cache, v_cache, block_table, seq_lens, cu, table, interleaved
 
 
 def attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, ids, block, scale):
-    """float64 out [B, Hq, D], lse [B, Hq], and the sizes sum(p |v|) and sum |q||k| scale behind them."""
+    """float64 out [B, Hq, D] and lse [B, Hq], and what bounds their float32 errors: per row, the largest
+    sum of a logit's absolute terms (each query element counted as the head's largest at least once),
+    sum(p |v|) per element, and keys * 448 * max(p v_scale)."""
     batch, hq, dim = q.shape
     groups = k_cache.shape[2]
     size, h = k_cache.shape[1], hq // groups
     out, size_o = (torch.zeros(batch, hq, dim, dtype=torch.float64) for _ in range(2))
-    lse, size_s = (torch.full((batch, hq), -math.inf, dtype=torch.float64) for _ in range(2))
+    lse = torch.full((batch, hq), -math.inf, dtype=torch.float64)
+    size_s, size_w, keys = (torch.zeros(batch, hq, dtype=torch.float64) for _ in range(3))
     for b, n in enumerate(seq_lens.tolist()):
         for g in range(groups):
             chosen = [i for i in dict.fromkeys(ids[b, g].tolist()) if i >= 0 and i * block < n]
-            if not chosen or n <= 0:
+            tok = [t for i in chosen for t in range(i * block, min((i + 1) * block, n))
+                   if t // size < block_table.shape[1] and 0 <= int(block_table[b, t // size]) < k_cache.shape[0]]
+            if not tok:
                 continue
-            tok = torch.cat([torch.arange(i * block, min((i + 1) * block, n)) for i in chosen])
+            tok = torch.tensor(tok)
             page, row = block_table[b].long()[tok // size], tok % size
             kk = k_cache[page, row, g].float().double() * k_scale[page, g].double()[:, None]
-            vv = v_cache[page, row, g].float().double() * v_scale[page, g].double()[:, None]
+            vs = v_scale[page, g].double()
+            vv = v_cache[page, row, g].float().double() * vs[:, None]
             rows = slice(g * h, (g + 1) * h)
             x = q[b, rows].double()
             logit = x @ kk.T * scale
@@ -96,5 +102,8 @@ def attend(q, k_cache, v_cache, k_scale, v_scale, block_table, seq_lens, ids, bl
             p = torch.exp(logit - lse[b, rows][:, None])
             out[b, rows] = p @ vv
             size_o[b, rows] = p @ vv.abs()
-            size_s[b, rows] = (x.abs() @ kk.abs().T * abs(scale)).amax(-1)
-    return out, lse, size_o, size_s
+            largest = x.abs().amax(-1, keepdim=True)
+            size_s[b, rows] = ((x.abs() @ kk.abs().T + largest * kk.abs().sum(-1)) * abs(scale)).amax(-1)
+            size_w[b, rows] = (p * vs).amax(-1) * 448 * len(tok)
+            keys[b, rows] = len(tok)
+    return out, lse, size_s, size_o, size_w, keys
