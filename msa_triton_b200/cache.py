@@ -93,7 +93,9 @@ def m3_cache_append(
             raise ValueError("k_cache and v_cache must share their pages and dtype")
     elif v_scale is not None:
         raise ValueError("v_scale belongs to an 8-bit cache")
-    batch = seq_lens.shape[0] if seq_lens.ndim == 1 else -1
+    if seq_lens.ndim != 1:
+        raise ValueError("seq_lens must be int32 [B]")
+    batch = seq_lens.shape[0]
     _check_paged(block_table, seq_lens, batch, k.device)
     if cu_seqlens is None:
         if total != batch:
