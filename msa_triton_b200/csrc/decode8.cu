@@ -6,15 +6,16 @@
 //   l = sum_j 2^(x_j - M)                                lse = (M + log2 l) ln 2
 //
 // HBM-bound: a key costs 2 D bytes and 4 h D flops for its group's h query heads. The work of a key is
-// small but not free (each byte has to become a number), so both products run on mma.sync m16n8k16 (heads
-// are the 16 rows; tcgen05's 128-row tiles would be 7/8 empty) and every byte is read from shared memory
-// once, into the register that the instruction takes: no transposition.
-//   * S = Q K^T: B's fragment wants pairs of neighbouring dims of one key; a lane (key n = lane / 4,
-//     j = lane % 4) loads 16 bytes of its key's row, and the dims are renumbered so that its k index runs
+// small but not free (each byte has to become a number), so both products run on mma.sync m16n8k16, keys
+// or dims as the 16 rows and heads as the 8 columns (tcgen05's 128-row tiles would wait for 128 keys of one
+// warp), and every byte is read from shared memory once, into the register that the instruction takes:
+//   * S^T = K Q^T: A's fragment wants pairs of neighbouring dims of the keys n and n + 8; a lane (n = lane / 4,
+//     j = lane % 4) reads 16 bytes of a key's row, and the dims are renumbered so that its k index runs
 //     over them (Q's fragment is renumbered the same way).
-//   * O = P V: B's fragment wants pairs of neighbouring keys of one dim; a lane loads the same 16 dims of
-//     the keys 2j, 2j + 1, 2j + 8, 2j + 9 and interleaves them two bytes at a time. The column of an
-//     8-wide tile t is renumbered to dim 16 n + t.
+//   * O^T = V^T P^T: A's fragment wants pairs of neighbouring keys of one dim; a lane reads the same 16 dims
+//     of the keys 2j, 2j + 1, 2j + 8, 2j + 9 and interleaves them two bytes at a time. Rows n and n + 8 of
+//     tile t are renumbered to the dims 16 n + 2 t and 16 n + 2 t + 1. P^T's fragment is S^T's after
+//     movmatrix.
 // e4m3 fits fp16 exactly, so the operands are fp16: K and V exact; q divided by a power of two per head
 // (exact but for elements 2^-14 below the head's largest, which keep 2^-25 of it); the weights rounded to
 // 11 bits, which adds to a bf16 output less than its own rounding. float32 inputs take both q and the
@@ -55,8 +56,16 @@ struct Params {
   float* lse;
   int64_t num_pages;
   int q_heads, groups, dim, page_size, max_pages, topk, block, splits, dtype;
+  uint32_t page_mul, page_shift;  // division by page_size, see page_of
   float scale_log2;
+  bool uniform;  // 16 keys in a row never leave a page
 };
+
+// token / page_size for 0 <= token < 2^31: with s = ceil(log2 d) and mul = floor(2^32 (2^s - d) / d) + 1,
+// (mulhi(n, mul) + n) >> s is the exact quotient of every 32-bit n, and the sum does not overflow below 2^31.
+__device__ __forceinline__ int page_of(const Params& p, int token) {
+  return (int)((__umulhi((uint32_t)token, p.page_mul) + (uint32_t)token) >> p.page_shift);
+}
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -67,15 +76,11 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
       : "r"(a0), "r"(a1), "r"(a2), "r"(a3), "r"(b0), "r"(b1));
 }
 
-// With at most 8 heads the rows 8..15 are empty: their accumulators are never kept.
-__device__ __forceinline__ void mma(float (&d)[2], uint32_t a0, uint32_t, uint32_t a2, uint32_t, uint32_t b0,
-                                    uint32_t b1) {
-  asm volatile(
-      "{\n\t.reg .f32 x, y;\n\t"
-      "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, x, y}, {%2, %3, %4, %3}, {%5, %6}, "
-      "{%0, %1, %7, %7};\n\t}"
-      : "+f"(d[0]), "+f"(d[1])
-      : "r"(a0), "r"(0), "r"(a2), "r"(b0), "r"(b1), "f"(0.f));
+// The transposed 8 x 8 matrix of 16-bit elements, row lane / 4, columns 2 (lane % 4) and the next.
+__device__ __forceinline__ uint32_t transpose8(uint32_t x) {
+  uint32_t y;
+  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  return y;
 }
 
 __device__ __forceinline__ uint32_t pack_half2(float a, float b) {
@@ -144,13 +149,28 @@ __device__ __forceinline__ void store_any(void* p, int64_t i, int dtype, float x
   else reinterpret_cast<float*>(p)[i] = x;
 }
 
-__device__ __forceinline__ float quad_max(float x) {
-  x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 1));
-  return fmaxf(x, __shfl_xor_sync(0xffffffffu, x, 2));
+// 2^x and log2 x by the special function unit (2 ulp; subnormal results are zero: a weight 2^-126 of the largest).
+__device__ __forceinline__ float fast_exp2(float x) {
+  float y;
+  asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
 }
-__device__ __forceinline__ float quad_sum(float x) {
-  x += __shfl_xor_sync(0xffffffffu, x, 1);
-  return x + __shfl_xor_sync(0xffffffffu, x, 2);
+__device__ __forceinline__ float fast_log2(float x) {
+  float y;
+  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
+  return y;
+}
+
+// Over the eight lanes that share lane % 4.
+__device__ __forceinline__ float column_max(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) x = fmaxf(x, __shfl_xor_sync(0xffffffffu, x, o));
+  return x;
+}
+__device__ __forceinline__ float column_sum(float x) {
+#pragma unroll
+  for (int o = 4; o < 32; o <<= 1) x += __shfl_xor_sync(0xffffffffu, x, o);
+  return x;
 }
 
 __device__ __forceinline__ uint32_t cluster_address(uint32_t local, uint32_t rank) {
@@ -161,6 +181,11 @@ __device__ __forceinline__ uint32_t cluster_address(uint32_t local, uint32_t ran
 __device__ __forceinline__ float load_cluster(uint32_t at) {
   float x;
   asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at));
+  return x;
+}
+__device__ __forceinline__ float4 load_cluster4(uint32_t at) {
+  float4 x;
+  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at));
   return x;
 }
 __device__ __forceinline__ void cluster_sync() {
@@ -174,11 +199,19 @@ struct Layout {
   static constexpr int kStage = 2 * kTile * DP + 2 * kTile * 4 + 16;
   static constexpr int kRing = kStages * kStage + 32 * 4;
   static constexpr int kRows = 8 * HR;
-  static constexpr int kPart = (kRows * DP + 3 * kRows) * 4;
+  static constexpr int kPitch = DP + 4;  // floats; with part_at, no bank twice when a warp stores its rows
+  static constexpr int kStats = kRows * kPitch;  // then m_soft, m_val, l of each row; the block's after its own
+  static constexpr int kPart = (kStats + 6 * kRows) * 4;
   static constexpr int kBytes = ((kRing > kPart ? kRing : kPart) + 127) / 128 * 128;
 };
 
-// DP: head dim rounded up to 64, 128 or 256. HR: head rows a lane holds (1: up to 8 heads, 2: up to 16).
+// Float offset of the four dims 4 i .. 4 i + 3 of a row of the partial result.
+template <int DP, int HR>
+__device__ __forceinline__ int part_at(int row, int i) {
+  return row * Layout<DP, HR>::kPitch + 4 * (i ^ ((i >> 2) & 1));
+}
+
+// DP: head dim rounded up to 64, 128 or 256. HR: tiles of 8 heads (1 or 2).
 // SPLIT: float32 inputs. VEC: rows are 16-byte aligned and dim is a multiple of 16 (other shapes all run the
 // 16-row float32 form, which is right for every type and head count).
 template <int DP, int HR, bool SPLIT, bool VEC>
@@ -189,8 +222,8 @@ decode8_kernel(const __grid_constant__ Params p) {
   constexpr int kKC = DP / 64;      // 16-byte units of a key row per lane
   constexpr int kVB = DP / 8 < 16 ? DP / 8 : 16;  // bytes of a value row per lane and unit
   constexpr int kVC = DP / 8 / kVB;               // units
-  constexpr int kTiles = DP / 8;                  // 8-wide output tiles
-  constexpr int kKN = kTile / 8;                  // key groups of S
+  constexpr int kTiles = DP / 16;                 // 16-dim output tiles
+  constexpr int kKT = kTile / 16;                 // 16-key tiles of S
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, j = lane & 3;
   const int split = blockIdx.x % p.splits, bg = blockIdx.x / p.splits;
@@ -200,7 +233,7 @@ decode8_kernel(const __grid_constant__ Params p) {
   const int64_t q_row = (int64_t)b * p.q_heads + (int64_t)g * h_all + h0;
   // ---- queries: fragments of q / 2^e, and the factor 2^e * scale * log2(e) of each row
   uint32_t qa[HR][kSteps][2], qb[SPLIT ? HR : 1][SPLIT ? kSteps : 1][2];
-  float qf[HR];
+  float qf[HR][2];  // of the heads 8 r + 2 j + e, the columns of this lane
 #pragma unroll
   for (int r = 0; r < HR; ++r) {
     const int head = n + 8 * r;
@@ -213,12 +246,15 @@ decode8_kernel(const __grid_constant__ Params p) {
         x[c][i] = head < h && d < p.dim ? load_any(p.q, (q_row + head) * p.dim + d, p.dtype) : 0.f;
         top = fmaxf(top, fabsf(x[c][i]));
       }
-    top = quad_max(top);
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // 2^e with top < 2^(e+1); nothing is scaled in an all-zero, subnormal or infinite row
     const uint32_t e = __float_as_uint(top) >> 23;
     const bool scaled = e >= 2 && e <= 252;
     const float inv = scaled ? __uint_as_float((254 - e) << 23) : 1.f;
-    qf[r] = p.scale_log2 * (scaled ? __uint_as_float(e << 23) : 1.f);
+    const float f = p.scale_log2 * (scaled ? __uint_as_float(e << 23) : 1.f);
+    qf[r][0] = __shfl_sync(0xffffffffu, f, 8 * j);
+    qf[r][1] = __shfl_sync(0xffffffffu, f, 8 * j + 4);
 #pragma unroll
     for (int c = 0; c < kKC; ++c)
 #pragma unroll
@@ -231,13 +267,16 @@ decode8_kernel(const __grid_constant__ Params p) {
         }
   }
   // ---- running state
-  float o[kTiles][2 * HR], m_soft[HR], m_val[HR], l[HR];
+  float o[HR][kTiles][4], m_soft[HR][2], m_val[HR][2], l[HR][2];
 #pragma unroll
-  for (int t = 0; t < kTiles; ++t)
+  for (int r = 0; r < HR; ++r) {
 #pragma unroll
-    for (int i = 0; i < 2 * HR; ++i) o[t][i] = 0.f;
+    for (int t = 0; t < kTiles; ++t)
 #pragma unroll
-  for (int r = 0; r < HR; ++r) m_soft[r] = m_val[r] = -INFINITY, l[r] = 0.f;
+      for (int i = 0; i < 4; ++i) o[r][t][i] = 0.f;
+#pragma unroll
+    for (int e = 0; e < 2; ++e) m_soft[r][e] = m_val[r][e] = -INFINITY, l[r][e] = 0.f;
+  }
 
   uint8_t* mine = smem + warp * L::kBytes;
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(mine);
@@ -267,7 +306,7 @@ decode8_kernel(const __grid_constant__ Params p) {
       const int slot = tile / per_block, in_block = (tile - slot * per_block) * kTile + lane;
       const int64_t token = (int64_t)slots[slot] * p.block + in_block;
       if (in_block >= p.block || token > pos) return;
-      const int logical = (int)token / p.page_size;  // token <= pos fits 32 bits
+      const int logical = page_of(p, (int)token);  // token <= pos fits 32 bits
       row_in_page = (int)token - logical * p.page_size;
       if (logical < p.max_pages) page = p.block_table[(int64_t)b * p.max_pages + logical];
     };
@@ -280,20 +319,38 @@ decode8_kernel(const __grid_constant__ Params p) {
         const int64_t k_off = here ? page * p.k.ps + row_in_page * p.k.ts + g * p.k.hs : 0;
         const int64_t v_off = here ? page * p.v.ps + row_in_page * p.v.ts + g * p.v.hs : 0;
         constexpr int kUnits = DP / 16, kStep = 32 / kUnits;  // units of a row, rows of a step
-        const int unit = lane % kUnits;
-#pragma unroll(VEC ? kTile / kStep : 1)
-        for (int i = 0; i < kTile / kStep; ++i) {
-          const int row = i * kStep + lane / kUnits;
-          const uint8_t* kr = p.k.p + __shfl_sync(0xffffffffu, k_off, row);
-          const uint8_t* vr = p.v.p + __shfl_sync(0xffffffffu, v_off, row);
-          const bool wanted = (seen >> row & 1) && unit * 16 < p.dim;
-          const uint32_t kd = base + key_unit<DP>(row, unit), vd = base + kTile * DP + value_unit<DP>(row, unit);
-          if (VEC) {
-            cp_async16(kd, wanted ? kr + unit * 16 : p.k.p, wanted);
-            cp_async16(vd, wanted ? vr + unit * 16 : p.v.p, wanted);
-          } else {
-            copy_bytes(kd, kr, unit * 16, p.dim, wanted);
-            copy_bytes(vd, vr, unit * 16, p.dim, wanted);
+        const int unit = lane % kUnits, sub = lane / kUnits;
+        if (VEC && p.uniform && seen == 0xffffffffu) {
+          // two runs of 16 rows, each at a fixed stride
+          const bool inside = unit * 16 < p.dim;
+#pragma unroll
+          for (int s = 0; s < 2; ++s) {
+            const uint8_t* kr = p.k.p + __shfl_sync(0xffffffffu, k_off, 16 * s) + sub * p.k.ts + unit * 16;
+            const uint8_t* vr = p.v.p + __shfl_sync(0xffffffffu, v_off, 16 * s) + sub * p.v.ts + unit * 16;
+#pragma unroll
+            for (int i = 0; i < 16 / kStep; ++i) {
+              const int row = 16 * s + i * kStep + sub;
+              cp_async16(base + key_unit<DP>(row, unit), inside ? kr : p.k.p, inside);
+              cp_async16(base + kTile * DP + value_unit<DP>(row, unit), inside ? vr : p.v.p, inside);
+              kr += kStep * p.k.ts;
+              vr += kStep * p.v.ts;
+            }
+          }
+        } else {
+#pragma unroll 1
+          for (int i = 0; i < kTile / kStep; ++i) {
+            const int row = i * kStep + sub;
+            const uint8_t* kr = p.k.p + __shfl_sync(0xffffffffu, k_off, row);
+            const uint8_t* vr = p.v.p + __shfl_sync(0xffffffffu, v_off, row);
+            const bool wanted = (seen >> row & 1) && unit * 16 < p.dim;
+            const uint32_t kd = base + key_unit<DP>(row, unit), vd = base + kTile * DP + value_unit<DP>(row, unit);
+            if (VEC) {
+              cp_async16(kd, wanted ? kr + unit * 16 : p.k.p, wanted);
+              cp_async16(vd, wanted ? vr + unit * 16 : p.v.p, wanted);
+            } else {
+              copy_bytes(kd, kr, unit * 16, p.dim, wanted);
+              copy_bytes(vd, vr, unit * 16, p.dim, wanted);
+            }
           }
         }
         const int64_t at = here ? (int64_t)page * p.groups + g : 0;
@@ -317,97 +374,129 @@ decode8_kernel(const __grid_constant__ Params p) {
       cp_async_wait<kStages - 1>();
       __syncwarp();
       const uint32_t base_k = ring + stage * L::kStage, base_v2 = base_k + kTile * DP;
-      const float* scales = reinterpret_cast<const float*>(mine + stage * L::kStage + 2 * kTile * DP);
+      float* scales = reinterpret_cast<float*>(mine + stage * L::kStage + 2 * kTile * DP);
       const uint32_t now = *reinterpret_cast<const uint32_t*>(scales + 2 * kTile);
       if (now == 0) {  // no key of this tile is attended (behind the newest token)
         __syncwarp();
         continue;
       }
-      // ---- S
-      float x[kKN][2 * HR];
+      scales[kTile + lane] = fast_log2(scales[kTile + lane]);
+      __syncwarp();
+      // ---- S^T: x[kt][r][2 a + e] is key 16 kt + n + 8 a, head 8 r + 2 j + e
+      float x[kKT][HR][4];
 #pragma unroll
-      for (int i = 0; i < kKN; ++i) {
+      for (int kt = 0; kt < kKT; ++kt) {
 #pragma unroll
-        for (int e = 0; e < 2 * HR; ++e) x[i][e] = 0.f;
+        for (int r = 0; r < HR; ++r)
+#pragma unroll
+          for (int i = 0; i < 4; ++i) x[kt][r][i] = 0.f;
 #pragma unroll
         for (int c = 0; c < kKC; ++c) {
-          const uint4 unit = lds128(base_k + key_unit<DP>(8 * i + n, 4 * c + j));
-          const uint32_t kw[4] = {unit.x, unit.y, unit.z, unit.w};
+          const uint4 u0 = lds128(base_k + key_unit<DP>(16 * kt + n, 4 * c + j));
+          const uint4 u1 = lds128(base_k + key_unit<DP>(16 * kt + n + 8, 4 * c + j));
+          const uint32_t w0[4] = {u0.x, u0.y, u0.z, u0.w}, w1[4] = {u1.x, u1.y, u1.z, u1.w};
 #pragma unroll
           for (int w = 0; w < 4; ++w) {
-            const uint32_t b0 = e4m3::decode2((uint16_t)kw[w]), b1 = e4m3::decode2((uint16_t)(kw[w] >> 16));
+            uint32_t a0, a1, a2, a3;
+            e4m3::decode4(w0[w], a0, a2);
+            e4m3::decode4(w1[w], a1, a3);
             const int s = 4 * c + w;
-            mma(x[i], qa[0][s][0], qa[HR - 1][s][0], qa[0][s][1], qa[HR - 1][s][1], b0, b1);
-            if (SPLIT)
-              mma(x[i], qb[0][SPLIT ? s : 0][0], qb[SPLIT ? HR - 1 : 0][SPLIT ? s : 0][0], qb[0][SPLIT ? s : 0][1],
-                  qb[SPLIT ? HR - 1 : 0][SPLIT ? s : 0][1], b0, b1);
+#pragma unroll
+            for (int r = 0; r < HR; ++r) {
+              mma(x[kt][r], a0, a1, a2, a3, qa[r][s][0], qa[r][s][1]);
+              if (SPLIT) mma(x[kt][r], a0, a1, a2, a3, qb[SPLIT ? r : 0][SPLIT ? s : 0][0], qb[SPLIT ? r : 0][SPLIT ? s : 0][1]);
+            }
           }
         }
       }
       // ---- softmax weights
-      float top[HR], top_v[HR];
+      float top[HR][2], top_v[HR][2], shift[kKT][2];
 #pragma unroll
-      for (int r = 0; r < HR; ++r) top[r] = m_soft[r], top_v[r] = m_val[r];
-      float shift[kKN][2];
+      for (int r = 0; r < HR; ++r)
 #pragma unroll
-      for (int i = 0; i < kKN; ++i)
+        for (int e = 0; e < 2; ++e) top[r][e] = top_v[r][e] = -INFINITY;
 #pragma unroll
-        for (int e = 0; e < 2; ++e) {
-          const int key = 8 * i + 2 * j + e;
+      for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+        for (int a = 0; a < 2; ++a) {
+          const int key = 16 * kt + n + 8 * a;
           const float f = scales[key];
-          shift[i][e] = log2f(scales[kTile + key]);
+          shift[kt][a] = scales[kTile + key];
 #pragma unroll
-          for (int r = 0; r < HR; ++r) {
-            float& y = x[i][2 * r + e];
-            y = now >> key & 1 ? y * (qf[r] * f) : -INFINITY;
-            top[r] = fmaxf(top[r], y);
-            top_v[r] = fmaxf(top_v[r], y + shift[i][e]);
-          }
+          for (int r = 0; r < HR; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) x[kt][r][2 * a + e] *= qf[r][e] * f;
         }
-      float base[HR], base_v[HR], alpha_v[HR];
+      if (now != 0xffffffffu) {
 #pragma unroll
-      for (int r = 0; r < HR; ++r) {
-        top[r] = quad_max(top[r]);
-        top_v[r] = quad_max(top_v[r]);
-        base[r] = top[r] == -INFINITY ? 0.f : top[r];
-        base_v[r] = top_v[r] == -INFINITY ? 0.f : top_v[r];
-        l[r] *= exp2f(m_soft[r] - base[r]);
-        alpha_v[r] = exp2f(m_val[r] - base_v[r]);
-        m_soft[r] = top[r];
-        m_val[r] = top_v[r];
+        for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+          for (int a = 0; a < 2; ++a)
+            if (!(now >> (16 * kt + n + 8 * a) & 1)) {
+#pragma unroll
+              for (int r = 0; r < HR; ++r) x[kt][r][2 * a] = x[kt][r][2 * a + 1] = -INFINITY;
+            }
       }
 #pragma unroll
-      for (int i = 0; i < kKN; ++i)
+      for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
-        for (int e = 0; e < 2; ++e)
+        for (int a = 0; a < 2; ++a)
 #pragma unroll
-          for (int r = 0; r < HR; ++r) {
-            const float y = x[i][2 * r + e];
-            l[r] += exp2f(y - base[r]);
-            x[i][2 * r + e] = exp2f(y + shift[i][e] - base_v[r]);
-          }
+          for (int r = 0; r < HR; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              top[r][e] = fmaxf(top[r][e], x[kt][r][2 * a + e]);
+              top_v[r][e] = fmaxf(top_v[r][e], x[kt][r][2 * a + e] + shift[kt][a]);
+            }
+      float base[HR][2], base_v[HR][2], alpha[HR][2];
       bool rescale = false;
 #pragma unroll
-      for (int r = 0; r < HR; ++r) rescale = rescale || alpha_v[r] != 1.f;
+      for (int r = 0; r < HR; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float ms = fmaxf(m_soft[r][e], column_max(top[r][e]));
+          const float mv = fmaxf(m_val[r][e], column_max(top_v[r][e]));
+          base[r][e] = ms == -INFINITY ? 0.f : ms;
+          base_v[r][e] = mv == -INFINITY ? 0.f : mv;
+          l[r][e] *= fast_exp2(m_soft[r][e] - base[r][e]);
+          alpha[r][e] = fast_exp2(m_val[r][e] - base_v[r][e]);
+          rescale = rescale || mv != m_val[r][e];
+          m_soft[r][e] = ms;
+          m_val[r][e] = mv;
+        }
+#pragma unroll
+      for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+        for (int a = 0; a < 2; ++a)
+#pragma unroll
+          for (int r = 0; r < HR; ++r)
+#pragma unroll
+            for (int e = 0; e < 2; ++e) {
+              float& y = x[kt][r][2 * a + e];
+              l[r][e] += fast_exp2(y - base[r][e]);
+              y = fast_exp2(y + shift[kt][a] - base_v[r][e]);
+            }
       if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
-        for (int d = 0; d < kTiles; ++d)
+        for (int r = 0; r < HR; ++r)
 #pragma unroll
-          for (int r = 0; r < HR; ++r) o[d][2 * r] *= alpha_v[r], o[d][2 * r + 1] *= alpha_v[r];
+          for (int t = 0; t < kTiles; ++t)
+#pragma unroll
+            for (int i = 0; i < 4; ++i) o[r][t][i] *= alpha[r][i & 1];
       }
-      // ---- O += P V
+      // ---- O^T += V^T P^T
 #pragma unroll
-      for (int s = 0; s < kTile / 16; ++s) {
-        uint32_t a[4], rest[4] = {};
+      for (int s = 0; s < kKT; ++s) {
+        uint32_t b[HR][2], rest[SPLIT ? HR : 1][2];
 #pragma unroll
-        for (int i = 0; i < 2; ++i)
+        for (int r = 0; r < HR; ++r)
 #pragma unroll
-          for (int r = 0; r < HR; ++r) {
-            const float y0 = x[2 * s + i][2 * r], y1 = x[2 * s + i][2 * r + 1];
-            a[2 * i + r] = pack_half2(y0, y1);
-            if (SPLIT) rest[2 * i + r] = pack_rest(y0, y1, a[2 * i + r]);
+          for (int a = 0; a < 2; ++a) {
+            const float y0 = x[s][r][2 * a], y1 = x[s][r][2 * a + 1];
+            const uint32_t packed = pack_half2(y0, y1);
+            b[r][a] = transpose8(packed);
+            if (SPLIT) rest[SPLIT ? r : 0][a] = transpose8(pack_rest(y0, y1, packed));
           }
-        if (HR == 1) a[1] = a[3] = 0;
 #pragma unroll
         for (int c = 0; c < kVC; ++c) {
           uint32_t vw[4][kVB / 4];
@@ -424,19 +513,19 @@ decode8_kernel(const __grid_constant__ Params p) {
           }
 #pragma unroll
           for (int w = 0; w < kVB / 4; ++w) {
-            // four dims of the keys (2j, 2j + 1) and (2j + 8, 2j + 9)
-            const uint32_t lo0 = __byte_perm(vw[0][w], vw[1][w], 0x5140);
-            const uint32_t lo1 = __byte_perm(vw[0][w], vw[1][w], 0x7362);
-            const uint32_t hi0 = __byte_perm(vw[2][w], vw[3][w], 0x5140);
-            const uint32_t hi1 = __byte_perm(vw[2][w], vw[3][w], 0x7362);
+            // four dims of the keys (2j, 2j + 1) and (2j + 8, 2j + 9): two tiles
 #pragma unroll
-            for (int d = 0; d < 4; ++d) {
-              const uint32_t lo = d < 2 ? lo0 : lo1, hi = d < 2 ? hi0 : hi1;
-              const uint32_t b0 = e4m3::decode2((uint16_t)(d & 1 ? lo >> 16 : lo));
-              const uint32_t b1 = e4m3::decode2((uint16_t)(d & 1 ? hi >> 16 : hi));
-              const int tile = c * kVB + 4 * w + d;
-              mma(o[tile], a[0], a[1], a[2], a[3], b0, b1);
-              if (SPLIT) mma(o[tile], rest[0], rest[1], rest[2], rest[3], b0, b1);
+            for (int half = 0; half < 2; ++half) {
+              const uint32_t pick = half ? 0x7362 : 0x5140;
+              uint32_t a0, a1, a2, a3;
+              e4m3::decode4(__byte_perm(vw[0][w], vw[1][w], pick), a0, a1);
+              e4m3::decode4(__byte_perm(vw[2][w], vw[3][w], pick), a2, a3);
+              const int t = c * (kVB / 2) + 2 * w + half;
+#pragma unroll
+              for (int r = 0; r < HR; ++r) {
+                mma(o[r][t], a0, a1, a2, a3, b[r][0], b[r][1]);
+                if (SPLIT) mma(o[r][t], a0, a1, a2, a3, rest[SPLIT ? r : 0][0], rest[SPLIT ? r : 0][1]);
+              }
             }
           }
         }
@@ -446,63 +535,119 @@ decode8_kernel(const __grid_constant__ Params p) {
     cp_async_wait<0>();
   }
 
-  // ---- the warp's partial result to its shared memory: o[row][DP], then m_soft, m_val, l of its rows
+  // ---- the warp's partial result to its shared memory
   constexpr int kRows = L::kRows;
   __syncwarp();
   float* part = reinterpret_cast<float*>(mine);
 #pragma unroll
-  for (int r = 0; r < HR; ++r) {
-    const float sum = quad_sum(l[r]);
-    const int row = n + 8 * r;
-    if (j == 0) {
-      part[kRows * DP + row] = m_soft[r];
-      part[kRows * DP + kRows + row] = m_val[r];
-      part[kRows * DP + 2 * kRows + row] = sum;
+  for (int r = 0; r < HR; ++r)
+#pragma unroll
+    for (int e = 0; e < 2; ++e) {
+      const float sum = column_sum(l[r][e]);
+      const int row = 8 * r + 2 * j + e;
+      if (n == 0) {
+        part[L::kStats + row] = m_soft[r][e];
+        part[L::kStats + kRows + row] = m_val[r][e];
+        part[L::kStats + 2 * kRows + row] = sum;
+      }
+      // rows n and n + 8 of tile (c, t) are the dims 128 c + kVB n + 2 t and the next
+#pragma unroll
+      for (int c = 0; c < kVC; ++c)
+#pragma unroll
+        for (int i = 0; i < kVB / 2; i += 2) {
+          const int t = c * (kVB / 2) + i;
+          *reinterpret_cast<float4*>(part + part_at<DP, HR>(row, (128 * c + kVB * n + 2 * i) / 4)) =
+              make_float4(o[r][t][e], o[r][t][2 + e], o[r][t + 1][e], o[r][t + 1][2 + e]);
+        }
     }
-    // column 2j + e of tile (c, t) is dim 128 c + kVB (2j + e) + t
-#pragma unroll
-    for (int c = 0; c < kVC; ++c)
-#pragma unroll
-      for (int e = 0; e < 2; ++e)
-#pragma unroll
-        for (int i = 0; i < kVB; i += 4)
-          *reinterpret_cast<float4*>(part + row * DP + 128 * c + kVB * (2 * j + e) + i) =
-              make_float4(o[c * kVB + i][2 * r + e], o[c * kVB + i + 1][2 * r + e], o[c * kVB + i + 2][2 * r + e],
-                          o[c * kVB + i + 3][2 * r + e]);
-  }
-  if (p.splits > 1) cluster_sync(); else __syncthreads();
+  __syncthreads();
 
-  // ---- merge: the cluster's threads share the output elements
-  const uint32_t here = (uint32_t)__cvta_generic_to_shared(smem);
-  for (int i = split * kWarps * 32 + threadIdx.x; i < h * DP; i += p.splits * kWarps * 32) {
-    const int row = i / DP, d = i - row * DP;
-    float top = -INFINITY, top_v = -INFINITY, sum = 0.f, acc = 0.f;
-    for (int s = 0; s < p.splits; ++s) {
-      const uint32_t base = cluster_address(here, s);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const uint32_t at = base + w * L::kBytes + 4 * (kRows * DP + row);
-        top = fmaxf(top, load_cluster(at));
-        top_v = fmaxf(top_v, load_cluster(at + 4 * kRows));
-      }
-    }
-    const float b0 = top == -INFINITY ? 0.f : top, bv = top_v == -INFINITY ? 0.f : top_v;
-    for (int s = 0; s < p.splits; ++s) {
-      const uint32_t base = cluster_address(here, s);
-#pragma unroll
-      for (int w = 0; w < kWarps; ++w) {
-        const uint32_t at = base + w * L::kBytes + 4 * (kRows * DP + row);
-        sum += load_cluster(at + 8 * kRows) * exp2f(load_cluster(at) - b0);
-        acc += load_cluster(base + w * L::kBytes + 4 * (row * DP + d)) * exp2f(load_cluster(at + 4 * kRows) - bv);
-      }
-    }
+  // Joins partial results (m_soft, m_val, l, o) of a row: what the first three become, and each one's
+  // factor for o.
+  struct Joined {
+    float m_soft = -INFINITY, m_val = -INFINITY, l = 0.f;
+  };
+  auto finish = [&](int row, int i, const Joined& s, float4 acc) {
     // no key: zero and -inf; a NaN sum stays one
-    const bool none = top == -INFINITY && sum == 0.f;
-    if (d < p.dim)
-      store_any(p.out, (q_row + row) * p.dim + d, p.dtype, none ? 0.f : acc * exp2f(bv - b0) / sum);
-    if (d == 0) p.lse[q_row + row] = none ? -INFINITY : (b0 + log2f(sum)) * 0.6931471805599453f;
+    const bool none = s.m_soft == -INFINITY && s.l == 0.f;
+    const float b0 = s.m_soft == -INFINITY ? 0.f : s.m_soft, bv = s.m_val == -INFINITY ? 0.f : s.m_val;
+    const float f = none ? 0.f : exp2f(bv - b0) / s.l;
+    const float v[4] = {acc.x, acc.y, acc.z, acc.w};
+#pragma unroll
+    for (int e = 0; e < 4; ++e)
+      if (4 * i + e < p.dim) store_any(p.out, (q_row + row) * p.dim + 4 * i + e, p.dtype, none ? 0.f : v[e] * f);
+    if (i == 0) p.lse[q_row + row] = none ? -INFINITY : (b0 + log2f(s.l)) * 0.6931471805599453f;
+  };
+
+  // ---- the block's warps: thread by thread in place, over the first warp's part
+  float* merged = reinterpret_cast<float*>(smem);
+  for (int at = threadIdx.x; at < h * (DP / 4); at += kWarps * 32) {
+    const int row = at / (DP / 4), i = at % (DP / 4);
+    Joined s;
+    float ms[kWarps], mv[kWarps];
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float* stats = reinterpret_cast<const float*>(smem + w * L::kBytes) + L::kStats + row;
+      ms[w] = stats[0], mv[w] = stats[kRows];
+      s.m_soft = fmaxf(s.m_soft, ms[w]);
+      s.m_val = fmaxf(s.m_val, mv[w]);
+    }
+    const float b0 = s.m_soft == -INFINITY ? 0.f : s.m_soft, bv = s.m_val == -INFINITY ? 0.f : s.m_val;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      const float* from = reinterpret_cast<const float*>(smem + w * L::kBytes);
+      s.l += from[L::kStats + 2 * kRows + row] * fast_exp2(ms[w] - b0);
+      const float4 v = *reinterpret_cast<const float4*>(from + part_at<DP, HR>(row, i));
+      const float f = fast_exp2(mv[w] - bv);
+      acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+    }
+    if (p.splits == 1) {
+      finish(row, i, s, acc);
+    } else {
+      *reinterpret_cast<float4*>(merged + part_at<DP, HR>(row, i)) = acc;
+      if (i == 0) {
+        merged[L::kStats + 3 * kRows + row] = s.m_soft;
+        merged[L::kStats + 4 * kRows + row] = s.m_val;
+        merged[L::kStats + 5 * kRows + row] = s.l;
+      }
+    }
   }
-  if (p.splits > 1) cluster_sync();  // the others may still read this block's memory
+  if (p.splits == 1) return;
+
+  // ---- the cluster's blocks: each takes its share of the output
+  cluster_sync();
+  const uint32_t local = (uint32_t)__cvta_generic_to_shared(smem);
+  for (int at = threadIdx.x * p.splits + split; at < h * (DP / 4); at += kWarps * 32 * p.splits) {
+    const int row = at / (DP / 4), i = at % (DP / 4);
+    float ms[kMaxSplits], mv[kMaxSplits], ls[kMaxSplits];
+    float4 v[kMaxSplits];
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r) {
+      ms[r] = mv[r] = -INFINITY, ls[r] = 0.f, v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
+      if (r < p.splits) {
+        const uint32_t from = cluster_address(local, r), stats = from + 4 * (L::kStats + 3 * kRows + row);
+        ms[r] = load_cluster(stats);
+        mv[r] = load_cluster(stats + 4 * kRows);
+        ls[r] = load_cluster(stats + 8 * kRows);
+        v[r] = load_cluster4(from + 4 * part_at<DP, HR>(row, i));
+      }
+    }
+    Joined s;
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r) s.m_soft = fmaxf(s.m_soft, ms[r]), s.m_val = fmaxf(s.m_val, mv[r]);
+    const float b0 = s.m_soft == -INFINITY ? 0.f : s.m_soft, bv = s.m_val == -INFINITY ? 0.f : s.m_val;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r) {
+      s.l += ls[r] * fast_exp2(ms[r] - b0);
+      const float f = fast_exp2(mv[r] - bv);
+      acc.x = fmaf(v[r].x, f, acc.x), acc.y = fmaf(v[r].y, f, acc.y);
+      acc.z = fmaf(v[r].z, f, acc.z), acc.w = fmaf(v[r].w, f, acc.w);
+    }
+    finish(row, i, s, acc);
+  }
+  cluster_sync();  // the others may still read this block's memory
 }
 
 template <int DP, int HR, bool SPLIT, bool VEC>
@@ -566,6 +711,10 @@ extern "C" int msa_decode_attn_e4m3(const void* q, int dtype, const void* k_cach
   const int64_t tiles = (int64_t)topk_blocks * ((block_size + kTile - 1) / kTile);
   p.splits = 1;
   while (p.splits < kMaxSplits && (int64_t)batch * groups * p.splits < 148 * 6 && p.splits * kWarps < tiles) p.splits *= 2;
+  p.page_shift = 0;
+  while (((uint32_t)1 << p.page_shift) < (uint32_t)page_size) ++p.page_shift;
+  p.page_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << p.page_shift) - page_size)) / page_size + 1);
+  p.uniform = page_size % 16 == 0 && block_size % 16 == 0;
   const bool vec = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(k_cache) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(v_cache) % 16 == 0 &&
                    (k_page_stride | k_slot_stride | k_head_stride | v_page_stride | v_slot_stride | v_head_stride) % 16 == 0;

@@ -38,15 +38,17 @@ __device__ __forceinline__ float decode1(uint8_t c) {
   return __half2float(__half(__nv_cvt_fp8_to_halfraw(c, __NV_E4M3)));
 }
 
-// Two codes (low byte first) to two halves: exact, e4m3's range lies inside fp16's.
-__device__ __forceinline__ uint32_t decode2(uint16_t c) {
-  const __half2_raw h = __nv_cvt_fp8x2_to_halfraw2(c, __NV_E4M3);
-  return (uint32_t)h.x | ((uint32_t)h.y << 16);
+// Four codes to two pairs of halves (low bytes first): exact, e4m3's range lies inside fp16's.
+__device__ __forceinline__ void decode4(uint32_t w, uint32_t& lo, uint32_t& hi) {
+  asm("{\n\t.reg .b16 x, y;\n\tmov.b32 {x, y}, %2;\n\tcvt.rn.f16x2.e4m3x2 %0, x;\n\tcvt.rn.f16x2.e4m3x2 %1, y;\n\t}"
+      : "=r"(lo), "=r"(hi)
+      : "r"(w));
 }
 
 // Four codes moved to another scale (ratio = old / new).
 __device__ __forceinline__ uint32_t rescale4(uint32_t w, float ratio) {
-  const uint32_t lo = decode2((uint16_t)w), hi = decode2((uint16_t)(w >> 16));
+  uint32_t lo, hi;
+  decode4(w, lo, hi);
   const float2 a = __half22float2(*reinterpret_cast<const __half2*>(&lo));
   const float2 b = __half22float2(*reinterpret_cast<const __half2*>(&hi));
   return encode4(a.x, a.y, b.x, b.y, ratio);
