@@ -138,15 +138,63 @@ __device__ __forceinline__ void copy_bytes(uint32_t dst, const uint8_t* row, int
   }
 }
 
-__device__ __forceinline__ float load_any(const void* p, int64_t i, int dtype) {
-  if (dtype == MSA_BF16) return __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(p)[i]);
-  if (dtype == MSA_F16) return __half2float(reinterpret_cast<const __half*>(p)[i]);
-  return reinterpret_cast<const float*>(p)[i];
+// 16 elements of a row from `d` on as floats, those past `dim` (or of an unwanted row) zero. VEC: 16-byte loads.
+template <bool VEC>
+__device__ __forceinline__ void load_q(float (&x)[16], const void* q, int64_t row, int d, int dim, int dtype,
+                                       bool wanted) {
+#pragma unroll
+  for (int i = 0; i < 16; ++i) x[i] = 0.f;
+  if (!wanted || d >= dim) return;
+  if (!VEC) {
+    for (int i = 0; i < 16 && d + i < dim; ++i) {
+      const int64_t at = row * dim + d + i;
+      x[i] = dtype == MSA_BF16 ? __bfloat162float(reinterpret_cast<const __nv_bfloat16*>(q)[at])
+             : dtype == MSA_F16 ? __half2float(reinterpret_cast<const __half*>(q)[at])
+                                : reinterpret_cast<const float*>(q)[at];
+    }
+    return;
+  }
+  const uint4* from = reinterpret_cast<const uint4*>(static_cast<const uint8_t*>(q) +
+                                                     (row * dim + d) * (dtype == MSA_F32 ? 4 : 2));
+  uint4 u[4];
+  u[0] = __ldg(from), u[1] = __ldg(from + 1);
+  if (dtype == MSA_F32) {
+    u[2] = __ldg(from + 2), u[3] = __ldg(from + 3);
+#pragma unroll
+    for (int i = 0; i < 4; ++i) {
+      x[4 * i] = __uint_as_float(u[i].x), x[4 * i + 1] = __uint_as_float(u[i].y);
+      x[4 * i + 2] = __uint_as_float(u[i].z), x[4 * i + 3] = __uint_as_float(u[i].w);
+    }
+    return;
+  }
+#pragma unroll
+  for (int i = 0; i < 8; ++i) {
+    const uint32_t w = i & 3 ? (i & 3) == 1 ? u[i / 4].y : (i & 3) == 2 ? u[i / 4].z : u[i / 4].w : u[i / 4].x;
+    const float2 f = dtype == MSA_BF16 ? __bfloat1622float2(*reinterpret_cast<const __nv_bfloat162*>(&w))
+                                       : __half22float2(*reinterpret_cast<const __half2*>(&w));
+    x[2 * i] = f.x, x[2 * i + 1] = f.y;
+  }
 }
-__device__ __forceinline__ void store_any(void* p, int64_t i, int dtype, float x) {
-  if (dtype == MSA_BF16) reinterpret_cast<__nv_bfloat16*>(p)[i] = __float2bfloat16_rn(x);
-  else if (dtype == MSA_F16) reinterpret_cast<__half*>(p)[i] = __float2half_rn(x);
-  else reinterpret_cast<float*>(p)[i] = x;
+
+// Four elements of the output from `d` on.
+template <bool VEC>
+__device__ __forceinline__ void store_out(void* out, int64_t row, int d, int dim, int dtype, float4 v) {
+  if (d >= dim) return;
+  const int64_t at = row * dim + d;
+  if (VEC) {
+    if (dtype == MSA_BF16) rope::store4(reinterpret_cast<__nv_bfloat16*>(out) + at, v.x, v.y, v.z, v.w);
+    else if (dtype == MSA_F16) rope::store4(reinterpret_cast<__half*>(out) + at, v.x, v.y, v.z, v.w);
+    else rope::store4(reinterpret_cast<float*>(out) + at, v.x, v.y, v.z, v.w);
+    return;
+  }
+  const float f[4] = {v.x, v.y, v.z, v.w};
+#pragma unroll
+  for (int e = 0; e < 4; ++e)
+    if (d + e < dim) {
+      if (dtype == MSA_BF16) reinterpret_cast<__nv_bfloat16*>(out)[at + e] = __float2bfloat16_rn(f[e]);
+      else if (dtype == MSA_F16) reinterpret_cast<__half*>(out)[at + e] = __float2half_rn(f[e]);
+      else reinterpret_cast<float*>(out)[at + e] = f[e];
+    }
 }
 
 // 2^x and log2 x by the special function unit (2 ulp; subnormal results are zero: a weight 2^-126 of the largest).
@@ -178,19 +226,12 @@ __device__ __forceinline__ uint32_t cluster_address(uint32_t local, uint32_t ran
   asm volatile("mapa.shared::cluster.u32 %0, %1, %2;" : "=r"(remote) : "r"(local), "r"(rank));
   return remote;
 }
-__device__ __forceinline__ float load_cluster(uint32_t at) {
-  float x;
-  asm volatile("ld.shared::cluster.f32 %0, [%1];" : "=f"(x) : "r"(at));
-  return x;
+__device__ __forceinline__ void store_cluster4(uint32_t at, float4 x) {
+  asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w)
+               : "memory");
 }
-__device__ __forceinline__ float4 load_cluster4(uint32_t at) {
-  float4 x;
-  asm volatile("ld.shared::cluster.v4.f32 {%0, %1, %2, %3}, [%4];" : "=f"(x.x), "=f"(x.y), "=f"(x.z), "=f"(x.w) : "r"(at));
-  return x;
-}
-__device__ __forceinline__ void cluster_sync() {
-  asm volatile("barrier.cluster.arrive.release.aligned;\n\tbarrier.cluster.wait.acquire.aligned;" ::: "memory");
-}
+__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Bytes of a warp's shared memory: its ring (keys, values, their scales, the mask of each tile), its list
 // of block ids; the partial result takes the same place at the end.
@@ -200,9 +241,11 @@ struct Layout {
   static constexpr int kRing = kStages * kStage + 32 * 4;
   static constexpr int kRows = 8 * HR;
   static constexpr int kPitch = DP + 4;  // floats; with part_at, no bank twice when a warp stores its rows
-  static constexpr int kStats = kRows * kPitch;  // then m_soft, m_val, l of each row; the block's after its own
-  static constexpr int kPart = (kStats + 6 * kRows) * 4;
+  static constexpr int kStats = kRows * kPitch;  // then m_soft, m_val, l of each row
+  static constexpr int kPart = (kStats + 3 * kRows) * 4;
   static constexpr int kBytes = ((kRing > kPart ? kRing : kPart) + 127) / 128 * 128;
+  // what the cluster's blocks send one another: their shares of o, then (m_soft, m_val, l, -) of each row
+  static constexpr int kInbox = kRows * DP * 4 + kMaxSplits * kRows * 16;
 };
 
 // Float offset of the four dims 4 i .. 4 i + 3 of a row of the partial result.
@@ -212,7 +255,7 @@ __device__ __forceinline__ int part_at(int row, int i) {
 }
 
 // DP: head dim rounded up to 64, 128 or 256. HR: tiles of 8 heads (1 or 2).
-// SPLIT: float32 inputs. VEC: rows are 16-byte aligned and dim is a multiple of 16 (other shapes all run the
+// SPLIT: float32 inputs. VEC: rows (q's and out's too) are 16-byte aligned and dim is a multiple of 16 (other shapes all run the
 // 16-row float32 form, which is right for every type and head count).
 template <int DP, int HR, bool SPLIT, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32, DP == 128 && HR == 1 && !SPLIT ? 3 : 1)
@@ -229,6 +272,7 @@ decode8_kernel(const __grid_constant__ Params p) {
   const int split = blockIdx.x % p.splits, bg = blockIdx.x / p.splits;
   const int b = bg / p.groups, g = bg - b * p.groups;
   const int h_all = p.q_heads / p.groups, h0 = blockIdx.y * 16, h = min(16, h_all - h0);
+  if (p.splits > 1) cluster_arrive();  // waited for before the first store to another block
   const int pos = p.seq_lens[b] - 1;
   const int64_t q_row = (int64_t)b * p.q_heads + (int64_t)g * h_all + h0;
   // ---- queries: fragments of q / 2^e, and the factor 2^e * scale * log2(e) of each row
@@ -239,13 +283,11 @@ decode8_kernel(const __grid_constant__ Params p) {
     const int head = n + 8 * r;
     float x[kKC][16], top = 0.f;
 #pragma unroll
-    for (int c = 0; c < kKC; ++c)
+    for (int c = 0; c < kKC; ++c) {
+      load_q<VEC>(x[c], p.q, q_row + head, 64 * c + 16 * j, p.dim, p.dtype, head < h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) {
-        const int d = 64 * c + 16 * j + i;
-        x[c][i] = head < h && d < p.dim ? load_any(p.q, (q_row + head) * p.dim + d, p.dtype) : 0.f;
-        top = fmaxf(top, fabsf(x[c][i]));
-      }
+      for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[c][i]));
+    }
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
     top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
     // 2^e with top < 2^(e+1); nothing is scaled in an all-zero, subnormal or infinite row
@@ -562,97 +604,77 @@ decode8_kernel(const __grid_constant__ Params p) {
     }
   __syncthreads();
 
-  // Joins partial results (m_soft, m_val, l, o) of a row: what the first three become, and each one's
-  // factor for o.
-  struct Joined {
-    float m_soft = -INFINITY, m_val = -INFINITY, l = 0.f;
-  };
-  auto finish = [&](int row, int i, const Joined& s, float4 acc) {
+  auto finish = [&](int row, int i, float m, float mv, float sum, float4 acc) {
     // no key: zero and -inf; a NaN sum stays one
-    const bool none = s.m_soft == -INFINITY && s.l == 0.f;
-    const float b0 = s.m_soft == -INFINITY ? 0.f : s.m_soft, bv = s.m_val == -INFINITY ? 0.f : s.m_val;
-    const float f = none ? 0.f : exp2f(bv - b0) / s.l;
-    const float v[4] = {acc.x, acc.y, acc.z, acc.w};
-#pragma unroll
-    for (int e = 0; e < 4; ++e)
-      if (4 * i + e < p.dim) store_any(p.out, (q_row + row) * p.dim + 4 * i + e, p.dtype, none ? 0.f : v[e] * f);
-    if (i == 0) p.lse[q_row + row] = none ? -INFINITY : (b0 + log2f(s.l)) * 0.6931471805599453f;
+    const bool none = m == -INFINITY && sum == 0.f;
+    const float f = none ? 0.f : exp2f((mv == -INFINITY ? 0.f : mv) - (m == -INFINITY ? 0.f : m)) / sum;
+    store_out<VEC>(p.out, q_row + row, 4 * i, p.dim, p.dtype,
+                   none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+    if (i == 0) p.lse[q_row + row] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m) + log2f(sum)) * 0.6931471805599453f;
+  };
+  auto add = [](float4& acc, const float4& v, float f) {
+    acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
   };
 
-  // ---- the block's warps: thread by thread in place, over the first warp's part
-  float* merged = reinterpret_cast<float*>(smem);
-  for (int at = threadIdx.x; at < h * (DP / 4); at += kWarps * 32) {
+  // ---- join the block's warps, four output elements a thread; with more blocks, send them to the block
+  // that finishes them (element at: block at % splits)
+  const uint32_t inbox = (uint32_t)__cvta_generic_to_shared(smem) + kWarps * L::kBytes;
+  const uint32_t inbox_stats = inbox + kRows * DP * 4;
+  const int elements = h * (DP / 4), share = (elements + p.splits - 1) / p.splits;
+  if (p.splits > 1) cluster_wait();  // every block of the cluster has started: its memory may be written
+  for (int at = threadIdx.x; at < elements; at += kWarps * 32) {
     const int row = at / (DP / 4), i = at % (DP / 4);
-    Joined s;
-    float ms[kWarps], mv[kWarps];
+    float m = -INFINITY, mv = -INFINITY, sum = 0.f, ms[kWarps], mvs[kWarps];
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float* stats = reinterpret_cast<const float*>(smem + w * L::kBytes) + L::kStats + row;
-      ms[w] = stats[0], mv[w] = stats[kRows];
-      s.m_soft = fmaxf(s.m_soft, ms[w]);
-      s.m_val = fmaxf(s.m_val, mv[w]);
+      ms[w] = stats[0], mvs[w] = stats[kRows];
+      m = fmaxf(m, ms[w]);
+      mv = fmaxf(mv, mvs[w]);
     }
-    const float b0 = s.m_soft == -INFINITY ? 0.f : s.m_soft, bv = s.m_val == -INFINITY ? 0.f : s.m_val;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float* from = reinterpret_cast<const float*>(smem + w * L::kBytes);
-      s.l += from[L::kStats + 2 * kRows + row] * fast_exp2(ms[w] - b0);
-      const float4 v = *reinterpret_cast<const float4*>(from + part_at<DP, HR>(row, i));
-      const float f = fast_exp2(mv[w] - bv);
-      acc.x = fmaf(v.x, f, acc.x), acc.y = fmaf(v.y, f, acc.y), acc.z = fmaf(v.z, f, acc.z), acc.w = fmaf(v.w, f, acc.w);
+      sum += from[L::kStats + 2 * kRows + row] * fast_exp2(ms[w] - (m == -INFINITY ? 0.f : m));
+      add(acc, *reinterpret_cast<const float4*>(from + part_at<DP, HR>(row, i)),
+          fast_exp2(mvs[w] - (mv == -INFINITY ? 0.f : mv)));
     }
     if (p.splits == 1) {
-      finish(row, i, s, acc);
+      finish(row, i, m, mv, sum, acc);
     } else {
-      *reinterpret_cast<float4*>(merged + part_at<DP, HR>(row, i)) = acc;
-      if (i == 0) {
-        merged[L::kStats + 3 * kRows + row] = s.m_soft;
-        merged[L::kStats + 4 * kRows + row] = s.m_val;
-        merged[L::kStats + 5 * kRows + row] = s.l;
-      }
+      store_cluster4(cluster_address(inbox, at % p.splits) + 16 * (split * share + at / p.splits), acc);
+      if (i < p.splits)  // DP / 4 > kMaxSplits
+        store_cluster4(cluster_address(inbox_stats, i) + 16 * (split * kRows + row), make_float4(m, mv, sum, 0.f));
     }
   }
   if (p.splits == 1) return;
 
-  // ---- the cluster's blocks: each takes its share of the output
-  cluster_sync();
-  const uint32_t local = (uint32_t)__cvta_generic_to_shared(smem);
-  for (int at = threadIdx.x * p.splits + split; at < h * (DP / 4); at += kWarps * 32 * p.splits) {
-    const int row = at / (DP / 4), i = at % (DP / 4);
-    float ms[kMaxSplits], mv[kMaxSplits], ls[kMaxSplits];
-    float4 v[kMaxSplits];
-#pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r) {
-      ms[r] = mv[r] = -INFINITY, ls[r] = 0.f, v[r] = make_float4(0.f, 0.f, 0.f, 0.f);
-      if (r < p.splits) {
-        const uint32_t from = cluster_address(local, r), stats = from + 4 * (L::kStats + 3 * kRows + row);
-        ms[r] = load_cluster(stats);
-        mv[r] = load_cluster(stats + 4 * kRows);
-        ls[r] = load_cluster(stats + 8 * kRows);
-        v[r] = load_cluster4(from + 4 * part_at<DP, HR>(row, i));
-      }
+  // ---- this block's elements, from its own memory: nobody reads it any more after this
+  cluster_arrive();
+  cluster_wait();
+  const float4* shares = reinterpret_cast<const float4*>(smem + kWarps * L::kBytes);
+  const float4* stats = shares + kRows * DP / 4;
+  for (int k = threadIdx.x; k * p.splits + split < elements; k += kWarps * 32) {
+    const int at = k * p.splits + split, row = at / (DP / 4), i = at % (DP / 4);
+    float m = -INFINITY, mv = -INFINITY, sum = 0.f;
+    for (int r = 0; r < p.splits; ++r) {
+      m = fmaxf(m, stats[r * kRows + row].x);
+      mv = fmaxf(mv, stats[r * kRows + row].y);
     }
-    Joined s;
-#pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r) s.m_soft = fmaxf(s.m_soft, ms[r]), s.m_val = fmaxf(s.m_val, mv[r]);
-    const float b0 = s.m_soft == -INFINITY ? 0.f : s.m_soft, bv = s.m_val == -INFINITY ? 0.f : s.m_val;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-#pragma unroll
-    for (int r = 0; r < kMaxSplits; ++r) {
-      s.l += ls[r] * fast_exp2(ms[r] - b0);
-      const float f = fast_exp2(mv[r] - bv);
-      acc.x = fmaf(v[r].x, f, acc.x), acc.y = fmaf(v[r].y, f, acc.y);
-      acc.z = fmaf(v[r].z, f, acc.z), acc.w = fmaf(v[r].w, f, acc.w);
+    for (int r = 0; r < p.splits; ++r) {
+      const float4 s = stats[r * kRows + row];
+      sum += s.z * fast_exp2(s.x - (m == -INFINITY ? 0.f : m));
+      add(acc, shares[r * share + k], fast_exp2(s.y - (mv == -INFINITY ? 0.f : mv)));
     }
-    finish(row, i, s, acc);
+    finish(row, i, m, mv, sum, acc);
   }
-  cluster_sync();  // the others may still read this block's memory
 }
 
 template <int DP, int HR, bool SPLIT, bool VEC>
 int launch(const Params& p, int batch, cudaStream_t st) {
-  const size_t smem = (size_t)kWarps * Layout<DP, HR>::kBytes;
+  const size_t smem = (size_t)kWarps * Layout<DP, HR>::kBytes + Layout<DP, HR>::kInbox;
   auto kernel = decode8_kernel<DP, HR, SPLIT, VEC>;
   if (smem > 48 * 1024)
     MSA_CUDA_RETURN(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
@@ -715,7 +737,8 @@ extern "C" int msa_decode_attn_e4m3(const void* q, int dtype, const void* k_cach
   while (((uint32_t)1 << p.page_shift) < (uint32_t)page_size) ++p.page_shift;
   p.page_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << p.page_shift) - page_size)) / page_size + 1);
   p.uniform = page_size % 16 == 0 && block_size % 16 == 0;
-  const bool vec = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(k_cache) % 16 == 0 &&
+  const bool vec = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
+                   reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(k_cache) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(v_cache) % 16 == 0 &&
                    (k_page_stride | k_slot_stride | k_head_stride | v_page_stride | v_slot_stride | v_head_stride) % 16 == 0;
   cudaStream_t st = as_stream(stream);
