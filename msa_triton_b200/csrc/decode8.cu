@@ -39,7 +39,7 @@ namespace {
 
 constexpr int kWarps = 4;
 constexpr int kTile = 32;      // keys a warp takes at a time
-constexpr int kStages = 2;
+constexpr int kStages = 2;     // tiles of a warp's ring
 constexpr int kMaxSplits = 8;  // blocks of a cluster
 
 struct Cache {
@@ -55,7 +55,7 @@ struct Params {
   void* out;
   float* lse;
   int64_t num_pages;
-  int q_heads, groups, dim, page_size, max_pages, topk, block, splits, dtype;
+  int q_heads, groups, dim, page_size, max_pages, topk, block, split_shift, dtype;  // 2^split_shift blocks a cluster
   uint32_t page_mul, page_shift;  // division by page_size, see page_of
   float scale_log2;
   bool uniform;  // 16 keys in a row never leave a page
@@ -269,45 +269,51 @@ decode8_kernel(const __grid_constant__ Params p) {
   constexpr int kKT = kTile / 16;                 // 16-key tiles of S
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, j = lane & 3;
-  const int split = blockIdx.x % p.splits, bg = blockIdx.x / p.splits;
+  const int splits = 1 << p.split_shift;
+  const int split = blockIdx.x & (splits - 1), bg = blockIdx.x >> p.split_shift;
   const int b = bg / p.groups, g = bg - b * p.groups;
   const int h_all = p.q_heads / p.groups, h0 = blockIdx.y * 16, h = min(16, h_all - h0);
-  if (p.splits > 1) cluster_arrive();  // waited for before the first store to another block
+  if (splits > 1) cluster_arrive();  // waited for before the first store to another block
+  const int32_t* ids = p.ids + (int64_t)bg * p.topk;
+  int id = lane < p.topk ? ids[lane] : -1;
   const int pos = p.seq_lens[b] - 1;
   const int64_t q_row = (int64_t)b * p.q_heads + (int64_t)g * h_all + h0;
   // ---- queries: fragments of q / 2^e, and the factor 2^e * scale * log2(e) of each row
-  uint32_t qa[HR][kSteps][2], qb[SPLIT ? HR : 1][SPLIT ? kSteps : 1][2];
-  float qf[HR][2];  // of the heads 8 r + 2 j + e, the columns of this lane
+  // (read after the first copies are on their way)
+  uint32_t qa[HR][kSteps][2] = {}, qb[SPLIT ? HR : 1][SPLIT ? kSteps : 1][2] = {};
+  float qf[HR][2] = {};  // of the heads 8 r + 2 j + e, the columns of this lane
+  auto load_queries = [&]() {
 #pragma unroll
-  for (int r = 0; r < HR; ++r) {
-    const int head = n + 8 * r;
-    float x[kKC][16], top = 0.f;
+    for (int r = 0; r < HR; ++r) {
+      const int head = n + 8 * r;
+      float x[kKC][16], top = 0.f;
 #pragma unroll
-    for (int c = 0; c < kKC; ++c) {
-      load_q<VEC>(x[c], p.q, q_row + head, 64 * c + 16 * j, p.dim, p.dtype, head < h);
+      for (int c = 0; c < kKC; ++c) {
+        load_q<VEC>(x[c], p.q, q_row + head, 64 * c + 16 * j, p.dim, p.dtype, head < h);
 #pragma unroll
-      for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[c][i]));
+        for (int i = 0; i < 16; ++i) top = fmaxf(top, fabsf(x[c][i]));
+      }
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
+      top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
+      // 2^e with top < 2^(e+1); nothing is scaled in an all-zero, subnormal or infinite row
+      const uint32_t e = __float_as_uint(top) >> 23;
+      const bool scaled = e >= 2 && e <= 252;
+      const float inv = scaled ? __uint_as_float((254 - e) << 23) : 1.f;
+      const float f = p.scale_log2 * (scaled ? __uint_as_float(e << 23) : 1.f);
+      qf[r][0] = __shfl_sync(0xffffffffu, f, 8 * j);
+      qf[r][1] = __shfl_sync(0xffffffffu, f, 8 * j + 4);
+#pragma unroll
+      for (int c = 0; c < kKC; ++c)
+#pragma unroll
+        for (int w = 0; w < 4; ++w)
+#pragma unroll
+          for (int u = 0; u < 2; ++u) {
+            const float a = x[c][4 * w + 2 * u] * inv, e2 = x[c][4 * w + 2 * u + 1] * inv;
+            qa[r][4 * c + w][u] = pack_half2(a, e2);
+            if (SPLIT) qb[r][4 * c + w][u] = pack_rest(a, e2, qa[r][4 * c + w][u]);
+          }
     }
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
-    top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-    // 2^e with top < 2^(e+1); nothing is scaled in an all-zero, subnormal or infinite row
-    const uint32_t e = __float_as_uint(top) >> 23;
-    const bool scaled = e >= 2 && e <= 252;
-    const float inv = scaled ? __uint_as_float((254 - e) << 23) : 1.f;
-    const float f = p.scale_log2 * (scaled ? __uint_as_float(e << 23) : 1.f);
-    qf[r][0] = __shfl_sync(0xffffffffu, f, 8 * j);
-    qf[r][1] = __shfl_sync(0xffffffffu, f, 8 * j + 4);
-#pragma unroll
-    for (int c = 0; c < kKC; ++c)
-#pragma unroll
-      for (int w = 0; w < 4; ++w)
-#pragma unroll
-        for (int u = 0; u < 2; ++u) {
-          const float a = x[c][4 * w + 2 * u] * inv, e2 = x[c][4 * w + 2 * u + 1] * inv;
-          qa[r][4 * c + w][u] = pack_half2(a, e2);
-          if (SPLIT) qb[r][4 * c + w][u] = pack_rest(a, e2, qa[r][4 * c + w][u]);
-        }
-  }
+  };
   // ---- running state
   float o[HR][kTiles][4], m_soft[HR][2], m_val[HR][2], l[HR][2];
 #pragma unroll
@@ -324,11 +330,10 @@ decode8_kernel(const __grid_constant__ Params p) {
   const uint32_t ring = (uint32_t)__cvta_generic_to_shared(mine);
   int32_t* slots = reinterpret_cast<int32_t*>(mine + kStages * L::kStage);  // this warp's compacted block ids
   const int per_block = (min(p.block, pos + 1) + kTile - 1) / kTile;
-  const int warps = p.splits * kWarps;
-  const int32_t* ids = p.ids + (int64_t)bg * p.topk;
+  const int warps = splits * kWarps;
   int before = 0;  // tiles of the earlier chunks of 32 ids
   for (int c0 = 0; c0 < p.topk && pos >= 0; c0 += 32) {
-    const int id = c0 + lane < p.topk ? ids[c0 + lane] : -1;
+    if (c0) id = c0 + lane < p.topk ? ids[c0 + lane] : -1;
     const uint32_t twins = __match_any_sync(0xffffffffu, id);
     bool valid = id >= 0 && id <= pos / p.block && (twins & ((1u << lane) - 1)) == 0;
     for (int i = 0; i < c0; ++i) valid = valid && ids[i] != id;
@@ -341,19 +346,23 @@ decode8_kernel(const __grid_constant__ Params p) {
     before += tiles;
 
     // Lane i looks up key i of a tile: its physical page (-1: no such key) and its row there.
-    int page = -1, row_in_page = 0;
+    struct Row {
+      int page, row;
+    };
     auto look_up = [&](int tile) {
-      page = -1;
-      if (tile >= tiles) return;
+      Row r{-1, 0};
+      if (tile >= tiles) return r;
       const int slot = tile / per_block, in_block = (tile - slot * per_block) * kTile + lane;
       const int64_t token = (int64_t)slots[slot] * p.block + in_block;
-      if (in_block >= p.block || token > pos) return;
+      if (in_block >= p.block || token > pos) return r;
       const int logical = page_of(p, (int)token);  // token <= pos fits 32 bits
-      row_in_page = (int)token - logical * p.page_size;
-      if (logical < p.max_pages) page = p.block_table[(int64_t)b * p.max_pages + logical];
+      r.row = (int)token - logical * p.page_size;
+      if (logical < p.max_pages) r.page = p.block_table[(int64_t)b * p.max_pages + logical];
+      return r;
     };
-    // Copies the tile that was looked up into a stage; always one group, empty behind the last tile.
-    auto issue = [&](int stage) {
+    // Copies a tile that was looked up into a stage; always one group, empty behind the last tile.
+    auto issue = [&](int stage, const Row& r) {
+      const int page = r.page, row_in_page = r.row;
       const bool here = page >= 0 && page < p.num_pages;
       const uint32_t seen = __ballot_sync(0xffffffffu, here);
       const uint32_t base = ring + stage * L::kStage;
@@ -403,17 +412,16 @@ decode8_kernel(const __grid_constant__ Params p) {
       cp_async_commit();
     };
 
-    look_up(first);
-#pragma unroll
-    for (int s = 0; s < kStages - 1; ++s) {
-      issue(s);
-      look_up(first + (s + 1) * warps);
-    }
+    // the table is read a tile ahead of the copies, the copies a tile ahead of the products
+    const Row now_row = look_up(first);
+    Row next = look_up(first + warps);
+    issue(0, now_row);
+    if (c0 == 0) load_queries();
     int stage = 0;
-    for (int t = first; t < tiles; t += warps, stage = stage + 1 == kStages ? 0 : stage + 1) {
-      issue(stage == 0 ? kStages - 1 : stage - 1);
-      look_up(t + kStages * warps);
-      cp_async_wait<kStages - 1>();
+    for (int t = first; t < tiles; t += warps, stage ^= 1) {
+      issue(stage ^ 1, next);
+      next = look_up(t + 2 * warps);
+      cp_async_wait<1>();
       __syncwarp();
       const uint32_t base_k = ring + stage * L::kStage, base_v2 = base_k + kTile * DP;
       float* scales = reinterpret_cast<float*>(mine + stage * L::kStage + 2 * kTile * DP);
@@ -620,8 +628,8 @@ decode8_kernel(const __grid_constant__ Params p) {
   // that finishes them (element at: block at % splits)
   const uint32_t inbox = (uint32_t)__cvta_generic_to_shared(smem) + kWarps * L::kBytes;
   const uint32_t inbox_stats = inbox + kRows * DP * 4;
-  const int elements = h * (DP / 4), share = (elements + p.splits - 1) / p.splits;
-  if (p.splits > 1) cluster_wait();  // every block of the cluster has started: its memory may be written
+  const int elements = h * (DP / 4), share = elements >> p.split_shift;  // DP / 4 is a multiple of kMaxSplits
+  if (splits > 1) cluster_wait();  // every block of the cluster has started: its memory may be written
   for (int at = threadIdx.x; at < elements; at += kWarps * 32) {
     const int row = at / (DP / 4), i = at % (DP / 4);
     float m = -INFINITY, mv = -INFINITY, sum = 0.f, ms[kWarps], mvs[kWarps];
@@ -640,34 +648,41 @@ decode8_kernel(const __grid_constant__ Params p) {
       add(acc, *reinterpret_cast<const float4*>(from + part_at<DP, HR>(row, i)),
           fast_exp2(mvs[w] - (mv == -INFINITY ? 0.f : mv)));
     }
-    if (p.splits == 1) {
+    if (splits == 1) {
       finish(row, i, m, mv, sum, acc);
     } else {
-      store_cluster4(cluster_address(inbox, at % p.splits) + 16 * (split * share + at / p.splits), acc);
-      if (i < p.splits)  // DP / 4 > kMaxSplits
+      store_cluster4(cluster_address(inbox, at & (splits - 1)) + 16 * (split * share + (at >> p.split_shift)), acc);
+      if (i < splits)
         store_cluster4(cluster_address(inbox_stats, i) + 16 * (split * kRows + row), make_float4(m, mv, sum, 0.f));
     }
   }
-  if (p.splits == 1) return;
+  if (splits == 1) return;
 
   // ---- this block's elements, from its own memory: nobody reads it any more after this
   cluster_arrive();
   cluster_wait();
   const float4* shares = reinterpret_cast<const float4*>(smem + kWarps * L::kBytes);
   const float4* stats = shares + kRows * DP / 4;
-  for (int k = threadIdx.x; k * p.splits + split < elements; k += kWarps * 32) {
-    const int at = k * p.splits + split, row = at / (DP / 4), i = at % (DP / 4);
+  for (int k = threadIdx.x; k < share; k += kWarps * 32) {
+    const int at = (k << p.split_shift) + split, row = at / (DP / 4), i = at % (DP / 4);
+    float4 part[kMaxSplits], s[kMaxSplits];
     float m = -INFINITY, mv = -INFINITY, sum = 0.f;
-    for (int r = 0; r < p.splits; ++r) {
-      m = fmaxf(m, stats[r * kRows + row].x);
-      mv = fmaxf(mv, stats[r * kRows + row].y);
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r) {
+      const int from = min(r, splits - 1);
+      s[r] = stats[from * kRows + row];
+      part[r] = shares[from * share + k];
+      m = fmaxf(m, s[r].x);
+      mv = fmaxf(mv, s[r].y);
     }
+    const float m0 = m == -INFINITY ? 0.f : m, mv0 = mv == -INFINITY ? 0.f : mv;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int r = 0; r < p.splits; ++r) {
-      const float4 s = stats[r * kRows + row];
-      sum += s.z * fast_exp2(s.x - (m == -INFINITY ? 0.f : m));
-      add(acc, shares[r * share + k], fast_exp2(s.y - (mv == -INFINITY ? 0.f : mv)));
-    }
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r)
+      if (r < splits) {
+        sum += s[r].z * fast_exp2(s[r].x - m0);
+        add(acc, part[r], fast_exp2(s[r].y - mv0));
+      }
     finish(row, i, m, mv, sum, acc);
   }
 }
@@ -679,13 +694,13 @@ int launch(const Params& p, int batch, cudaStream_t st) {
   if (smem > 48 * 1024)
     MSA_CUDA_RETURN(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(batch * p.groups * p.splits), (unsigned)ceil_div(p.q_heads / p.groups, 16));
+  cfg.gridDim = dim3((unsigned)(batch * p.groups) << p.split_shift, (unsigned)ceil_div(p.q_heads / p.groups, 16));
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
   cudaLaunchAttribute at;
   at.id = cudaLaunchAttributeClusterDimension;
-  at.val.clusterDim = {(unsigned)p.splits, 1, 1};
+  at.val.clusterDim = {1u << p.split_shift, 1, 1};
   cfg.attrs = &at;
   cfg.numAttrs = 1;
   MSA_CUDA_RETURN(cudaLaunchKernelEx(&cfg, kernel, p));
@@ -731,8 +746,9 @@ extern "C" int msa_decode_attn_e4m3(const void* q, int dtype, const void* k_cach
   p.scale_log2 = (float)(scale * 1.4426950408889634);
   // Blocks for a (request, group): until the chip is full, and no more warps than tiles.
   const int64_t tiles = (int64_t)topk_blocks * ((block_size + kTile - 1) / kTile);
-  p.splits = 1;
-  while (p.splits < kMaxSplits && (int64_t)batch * groups * p.splits < 148 * 6 && p.splits * kWarps < tiles) p.splits *= 2;
+  int splits = 1;
+  while (splits < kMaxSplits && (int64_t)batch * groups * splits < 148 * 6 && splits * kWarps < tiles)
+    splits *= 2, ++p.split_shift;
   p.page_shift = 0;
   while (((uint32_t)1 << p.page_shift) < (uint32_t)page_size) ++p.page_shift;
   p.page_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << p.page_shift) - page_size)) / page_size + 1);
