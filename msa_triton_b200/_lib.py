@@ -166,11 +166,29 @@ def call(name: str, *args) -> None:
 
 
 def ptr(t: torch.Tensor | None):
-    return None if t is None else c_void_p(t.data_ptr())
+    return None if t is None else t.data_ptr()
 
 
 def stream_of(t: torch.Tensor):
-    return c_void_p(torch.cuda.current_stream(t.device).cuda_stream)
+    """The current stream of the tensor's device (its handle, without a Stream object: decode
+    steps are launch-bound on the host, and this is read once per launch)."""
+    return torch._C._cuda_getCurrentRawStream(t.device.index)
+
+
+class _Here:
+    def __enter__(self):
+        return None
+
+    def __exit__(self, *exc):
+        return False
+
+
+_HERE = _Here()
+
+
+def device_of(t: torch.Tensor):
+    """``torch.cuda.device(t.device)``, or nothing where that device is the current one already."""
+    return _HERE if torch.cuda.current_device() == t.device.index else torch.cuda.device(t.device)
 
 
 def host_ints(t: torch.Tensor) -> list[int]:
@@ -188,12 +206,18 @@ def host_ints(t: torch.Tensor) -> list[int]:
     return list(buf[:n])
 
 
+_cuda_seen = False
+
+
 def require_cuda(*tensors: torch.Tensor) -> None:
+    global _cuda_seen
     for t in tensors:
-        if t.device.type != "cuda":
+        if not t.is_cuda:
             raise RuntimeError("msa_triton_b200 runs on CUDA devices only (no CPU fallback)")
-    if not torch.cuda.is_available():
-        raise RuntimeError("msa_triton_b200 needs a CUDA device")
+    if not _cuda_seen:
+        if not torch.cuda.is_available():
+            raise RuntimeError("msa_triton_b200 needs a CUDA device")
+        _cuda_seen = True
 
 # Tensor-core kernel families compiled into this build (flipped on as they land).
 HAS_TC_SCORE = True

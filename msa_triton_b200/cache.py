@@ -22,7 +22,7 @@ from __future__ import annotations
 import torch
 
 from . import _lib
-from ._lib import DTYPE_CODE, E4M3_CODE, call, ptr, stream_of
+from ._lib import DTYPE_CODE, E4M3_CODE, call, device_of, ptr, stream_of
 from .decode import CACHE_8BIT, _check_paged, check_scale
 from .qk_norm_rope import check_table, dense_rows
 
@@ -49,7 +49,6 @@ def _check_cache(name, x, cache, scale, device):
         span = stride * size
 
 
-@torch.no_grad()
 def m3_cache_append(
     k: torch.Tensor,
     v: torch.Tensor | None,
@@ -115,7 +114,7 @@ def m3_cache_append(
     pages, lens = block_table.contiguous(), seq_lens.contiguous()
     v_strides = (0, 0) if v is None else (vd.stride(0), vd.stride(1))
     v_cache_strides = (0, 0, 0) if v is None else v_cache.stride()[:3]
-    with torch.cuda.device(k.device):
+    with device_of(k):
         call("msa_cache_append", ptr(kd), ptr(vd), DTYPE_CODE[k.dtype], kd.stride(0), kd.stride(1), *v_strides,
              ptr(table), rows, rotary, int(interleaved), ptr(cu), ptr(pages), ptr(lens), batch, total,
              heads, dim, k_cache.shape[1], block_table.shape[1], k_cache.shape[0], ptr(k_cache), ptr(v_cache),

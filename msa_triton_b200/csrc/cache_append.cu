@@ -94,13 +94,13 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
   const LaneMap m = lane_map<INTER>(l, p.dim, s.rotary);
   const int h0 = chunk * (kSub * kRowsPerLane) + lane / LPR;
   const T* x = static_cast<const T*>(s.x) + (int64_t)t * s.x_ts;
-  Raw4<T> raw[kRowsPerLane][2];
+  Raw<T> raw[kRowsPerLane][2];
 #pragma unroll
   for (int i = 0; i < kRowsPerLane; ++i) {
     const int h = h0 + i * kSub;
     if (h < p.heads && m.active) {
-      raw[i][0] = load4(x + h * s.x_hs + m.a);
-      raw[i][1] = load4(x + h * s.x_hs + m.b);
+      raw[i][0] = load_run(x + h * s.x_hs + m.a);
+      raw[i][1] = load_run(x + h * s.x_hs + m.b);
     }
   }
   const int b = request_of(p, t);
@@ -117,17 +117,15 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
   for (int i = 0; i < kRowsPerLane; ++i) {
     const int h = h0 + i * kSub;
     if (h >= p.heads || !m.active) continue;
-    float a[4], e[4], v[8];
-    unpack4(raw[i][0], a);
-    unpack4(raw[i][1], e);
-    to_pairs<INTER>(a, e, v);
+    float v[8];
+    unpack_lane<INTER>(raw[i], v);
     if (!inside) {
 #pragma unroll
       for (int j = 0; j < 8; ++j) v[j] = nan_f32();
     } else if (rotated) {
-      rotate8(v, c, sn);
+      rotate_lane(v, c, sn);
     }
-    store8<INTER>(out + h * s.c_hs, m, v);
+    store_lane<INTER>(out + h * s.c_hs + m.a, out + h * s.c_hs + m.b, v);
   }
 }
 
@@ -208,11 +206,8 @@ __device__ __forceinline__ float amax8(const float (&v)[8], float acc) {
 // One row's eight values of a lane, rotated.
 template <typename T, bool INTER>
 __device__ __forceinline__ void rotated_row(const Params& p, const Half& s, const LaneMap& m, int l,
-                                            const Raw4<T> (&raw)[2], int64_t pos, float (&v)[8]) {
-  float a[4], b[4];
-  unpack4(raw[0], a);
-  unpack4(raw[1], b);
-  to_pairs<INTER>(a, b, v);
+                                            const Raw<T> (&raw)[2], int64_t pos, float (&v)[8]) {
+  unpack_lane<INTER>(raw, v);
   if (s.rotary == 0) return;
   if (pos >= p.table_rows) {
 #pragma unroll
@@ -220,7 +215,7 @@ __device__ __forceinline__ void rotated_row(const Params& p, const Half& s, cons
   } else if (m.rotated) {
     float c[4], sn[4];
     load_angles(p.table + pos * s.rotary, s.rotary, l, c, sn);
-    rotate8(v, c, sn);
+    rotate_lane(v, c, sn);
   }
 }
 
@@ -236,8 +231,8 @@ __global__ void __launch_bounds__(kWarps * 32) append8_token_kernel(const __grid
   const LaneMap m = lane_map<INTER>(l, p.dim, s.rotary);
   const bool mine = m.active && lane < LPR;
   const T* x = static_cast<const T*>(s.x) + (int64_t)b * s.x_ts + h * s.x_hs;
-  Raw4<T> raw[2] = {};
-  if (mine) raw[0] = load4(x + m.a), raw[1] = load4(x + m.b);
+  Raw<T> raw[2] = {};
+  if (mine) raw[0] = load_run(x + m.a), raw[1] = load_run(x + m.b);
   Task t;
   if (!find_task(p, b, t)) return;
   float* scale = s.scale + t.page * p.heads + h;
@@ -281,13 +276,13 @@ __global__ void __launch_bounds__(kWarps * 32) append8_page_kernel(const __grid_
   const T* x = static_cast<const T*>(s.x) + t.token * s.x_ts + h * s.x_hs;
   float* scale = s.scale + t.page * p.heads + h;
   const float old = *scale;
-  Raw4<T> raw[kKeep][2];
+  Raw<T> raw[kKeep][2];
 #pragma unroll
   for (int i = 0; i < kKeep; ++i) {
     const int r = r0 + i * kRows;
     if (r < t.n && m.active) {
-      raw[i][0] = load4(x + r * s.x_ts + m.a);
-      raw[i][1] = load4(x + r * s.x_ts + m.b);
+      raw[i][0] = load_run(x + r * s.x_ts + m.a);
+      raw[i][1] = load_run(x + r * s.x_ts + m.b);
     }
   }
   float amax = 0.f, v[8];
@@ -301,7 +296,7 @@ __global__ void __launch_bounds__(kWarps * 32) append8_page_kernel(const __grid_
   }
   for (int64_t r = r0 + kKeep * kRows; r < t.n; r += kRows) {
     if (!m.active) continue;
-    const Raw4<T> w[2] = {load4(x + r * s.x_ts + m.a), load4(x + r * s.x_ts + m.b)};
+    const Raw<T> w[2] = {load_run(x + r * s.x_ts + m.a), load_run(x + r * s.x_ts + m.b)};
     rotated_row<T, INTER>(p, s, m, l, w, t.pos + r, v);
     amax = amax8(v, amax);
   }
@@ -318,7 +313,7 @@ __global__ void __launch_bounds__(kWarps * 32) append8_page_kernel(const __grid_
   }
   for (int64_t r = r0 + kKeep * kRows; r < t.n; r += kRows) {
     if (!m.active) continue;
-    const Raw4<T> w[2] = {load4(x + r * s.x_ts + m.a), load4(x + r * s.x_ts + m.b)};
+    const Raw<T> w[2] = {load_run(x + r * s.x_ts + m.a), load_run(x + r * s.x_ts + m.b)};
     rotated_row<T, INTER>(p, s, m, l, w, t.pos + r, v);
     store_codes<INTER>(out + r * s.c_ts, m, v, inv);
   }
@@ -397,10 +392,10 @@ bool fast_shape(const Params& p, int halves, int dtype, bool quantised) {
   const int es = elem_size(dtype);
   for (int i = 0; i < halves; ++i) {
     const Half& s = p.half[i];
-    if (s.rotary % 8 || !rows_aligned(s.x, s.x_ts, s.x_hs, es)) return false;
+    if (s.rotary % 8 || !rows_aligned(s.x, s.x_ts, s.x_hs, es, kE * es)) return false;
     if (quantised) {
       if (reinterpret_cast<uintptr_t>(s.cache) % 16 || s.c_ps % 16 || s.c_ts % 16 || s.c_hs % 16) return false;
-    } else if (!rows_aligned(s.cache, s.c_ps, s.c_ts, es) || s.c_hs % 4) {
+    } else if (!rows_aligned(s.cache, s.c_ps, s.c_ts, es, kE * es) || s.c_hs % kE) {
       return false;
     }
   }

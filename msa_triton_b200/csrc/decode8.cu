@@ -181,13 +181,13 @@ template <bool VEC>
 __device__ __forceinline__ void store_out(void* out, int64_t row, int d, int dim, int dtype, float4 v) {
   if (d >= dim) return;
   const int64_t at = row * dim + d;
+  const float f[4] = {v.x, v.y, v.z, v.w};
   if (VEC) {
-    if (dtype == MSA_BF16) rope::store4(reinterpret_cast<__nv_bfloat16*>(out) + at, v.x, v.y, v.z, v.w);
-    else if (dtype == MSA_F16) rope::store4(reinterpret_cast<__half*>(out) + at, v.x, v.y, v.z, v.w);
-    else rope::store4(reinterpret_cast<float*>(out) + at, v.x, v.y, v.z, v.w);
+    if (dtype == MSA_BF16) rope::store_run(reinterpret_cast<__nv_bfloat16*>(out) + at, f);
+    else if (dtype == MSA_F16) rope::store_run(reinterpret_cast<__half*>(out) + at, f);
+    else rope::store_run(reinterpret_cast<float*>(out) + at, f);
     return;
   }
-  const float f[4] = {v.x, v.y, v.z, v.w};
 #pragma unroll
   for (int e = 0; e < 4; ++e)
     if (d + e < dim) {

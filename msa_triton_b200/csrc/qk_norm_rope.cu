@@ -12,9 +12,13 @@
 //
 // HBM-bound (about one operation per byte): each row is read once, held in registers for the
 // reduction and the rotation, and written once; the backward recomputes r from x (4 flops
-// an element) instead of storing it. q and k go through one launch. The weights' gradients
-// are summed in registers by persistent warps, then over a block's warps and the blocks in a
-// fixed order (no atomics, the same bits every run).
+// an element) instead of storing it. What is left to watch is the number of instructions (a warp has some
+// 300 issue slots to the 2 KB it reads and writes in the forward): arithmetic is done two floats at a time, w and the angles
+// are multiplied once for all the heads of a token, addresses advance by a fixed step. Warps stay and walk
+// over their tokens' heads, and hide one another's loads (a second set of registers for the next rows costs
+// more warps than it gains: 243 against 210 us forward). q and k go through one launch, each with blocks of its own. The weights' gradients are summed in
+// registers on the way, then over a block's warps and the blocks in a fixed order (no atomics, the same bits
+// every run).
 #include <algorithm>
 
 #include "rope_common.cuh"
@@ -24,11 +28,18 @@ namespace {
 
 using namespace rope;
 
-constexpr int kWarps = 8;
-constexpr int kRowsPerLane = 4;   // rows a lane loads before it uses the first (forward)
-constexpr int kRowsPerLaneB = 2;  // (backward: two tensors a row)
+constexpr int kWarps = 4;
 constexpr int kMaxDimFast = 256;
 constexpr int kMaxDim = 512;
+
+// Rows a lane takes at a time: 64 bytes of loads in flight for every type.
+template <typename T, bool BWD>
+constexpr int kRowsOf = 64 / (2 * kE * (int)sizeof(T)) / (BWD ? 2 : 1);
+
+// Blocks to an SM, by registers (72-76 forward, 96 backward). Measured at 71168 tokens of 40 heads of 128: 6 and 5
+// blocks 256 and 426 us; 7 (spilled) 254 and 465 us; 5 forward 286 us; 4 backward 430 us.
+template <bool BWD>
+constexpr int kResident = BWD ? 5 : 6;
 
 // One of q and k.
 struct Side {
@@ -38,6 +49,11 @@ struct Side {
   void* out;      // forward: y; backward: dx (may be null)
   int64_t x_ts, x_hs, g_ts, g_hs;  // strides in elements
   int heads;
+  // A warp takes `slots` rows at a time: heads of one token, `chunks` steps a token. An item of work is `span`
+  // steps of a token one after the other (`spans` items a token); the angles are loaded once for them. Where a
+  // token's heads would not fill a warp (flat), it takes that many rows in a row whatever their tokens.
+  uint32_t items, chunks, span, spans, first_block, blocks;
+  bool flat;
 };
 
 struct Params {
@@ -45,18 +61,26 @@ struct Params {
   const float* table;
   const int32_t* positions;  // or null: from cu
   const int32_t* cu;
-  float* partial;  // backward: [gridDim.x][2][dim], or null
+  float* partial;  // backward: [gridDim.x][dim] (any shape: [gridDim.x][2][dim]), or null
   int64_t table_rows, tokens;
   int nseq, dim, rotary, w_dtype;
-  uint32_t units, chunks, q_chunks;
   float eps, inv_dim;
   bool interleaved;
 };
 
-__device__ __forceinline__ int64_t position_of(const Params& p, int64_t t) {
-  if (p.positions) return p.positions[t];
-  return t - p.cu[find_sequence(p.cu, p.nseq, t)];
-}
+// Positions of tokens; the bounds of the last token's sequence are kept, so that a walk over the tokens
+// searches once a sequence (a search is a chain of dependent loads ahead of the table's row).
+struct Positions {
+  int64_t lo = 0, hi = 0;
+  __device__ __forceinline__ int64_t of(const Params& p, int64_t t) {
+    if (p.positions) return p.positions[t];
+    if (t < lo || t >= hi) {
+      const int s = find_sequence(p.cu, p.nseq, t);
+      lo = p.cu[s], hi = p.cu[s + 1];
+    }
+    return t - lo;
+  }
+};
 
 __device__ __forceinline__ float load_weight(const void* w, int i, int dtype) {
   if (dtype == MSA_F32) return reinterpret_cast<const float*>(w)[i];
@@ -65,11 +89,12 @@ __device__ __forceinline__ float load_weight(const void* w, int i, int dtype) {
 }
 
 template <bool INTER>
-__device__ __forceinline__ void load_weights(const void* w, int dtype, const LaneMap& m, float (&v)[8]) {
-  float a[4], b[4];
+__device__ __forceinline__ Lane weights_of(const void* w, int dtype, const LaneMap& m) {
+  float a[kE], b[kE], v[2 * kE];
 #pragma unroll
-  for (int i = 0; i < 4; ++i) a[i] = load_weight(w, m.a + i, dtype), b[i] = load_weight(w, m.b + i, dtype);
+  for (int i = 0; i < kE; ++i) a[i] = load_weight(w, m.a + i, dtype), b[i] = load_weight(w, m.b + i, dtype);
   to_pairs<INTER>(a, b, v);
+  return lane_of(v);
 }
 
 template <int LPR>
@@ -79,153 +104,263 @@ __device__ __forceinline__ float row_sum(float x) {
   return x;
 }
 
-// ------------------------------------------------------------------ forward
-// A warp takes 32 / LPR * kRowsPerLane heads of one token (q's or k's); the angles are
-// loaded once for them.
-template <typename T, int LPR, bool INTER>
-__global__ void __launch_bounds__(kWarps * 32) fwd_kernel(const __grid_constant__ Params p) {
-  constexpr int kSub = 32 / LPR;
-  const uint32_t unit = blockIdx.x * kWarps + (threadIdx.x >> 5);
-  if (unit >= p.units) return;
-  const uint32_t t = unit / p.chunks;
-  uint32_t chunk = unit - t * p.chunks;
-  const int lane = threadIdx.x & 31, l = lane % LPR;
-  const bool is_k = chunk >= p.q_chunks;
-  if (is_k) chunk -= p.q_chunks;
-  const Side& s = p.side[is_k];
-  const LaneMap m = lane_map<INTER>(l, p.dim, p.rotary);
-  const int h0 = chunk * (kSub * kRowsPerLane) + lane / LPR;
-  const T* x = static_cast<const T*>(s.x) + (int64_t)t * s.x_ts;
-  Raw4<T> raw[kRowsPerLane][2];
+// ------------------------------------------------------------------ rows in the lane layout
+// A lane's angles of one position, kE cosines and sines; lanes behind the rotated elements: 1 and 0.
+struct Angles {
+  float c[kE], s[kE];
+  bool inside = true;
+  __device__ __forceinline__ void load(const Params& p, Positions& positions, const LaneMap& m, int64_t t, int l) {
+    const int64_t pos = positions.of(p, t);
+    inside = pos >= 0 && pos < p.table_rows;
 #pragma unroll
-  for (int i = 0; i < kRowsPerLane; ++i) {
-    const int h = h0 + i * kSub;
-    if (h < s.heads && m.active) {
-      raw[i][0] = load4(x + h * s.x_hs + m.a);
-      raw[i][1] = load4(x + h * s.x_hs + m.b);
-    } else {
-      raw[i][0].u = raw[i][1].u = {};
+    for (int i = 0; i < kE; ++i) c[i] = 1.f, s[i] = 0.f;
+    if (inside && m.rotated) load_angles(p.table + pos * p.rotary, p.rotary, l, c, s);
+  }
+};
+
+// The forward rotation of w * x, of a pair's x = (a, b): (a c0 + b s1, b c1 + a s0).
+struct Turn {
+  F2 c0[kE / 2], s1[kE / 2], c1[kE / 2], s0[kE / 2];
+  __device__ __forceinline__ Turn(const Angles& t, const Lane& w) {
+#pragma unroll
+    for (int i = 0; i < kE / 2; ++i) {
+      const F2 c = pack2(t.c[2 * i], t.c[2 * i + 1]), s = pack2(t.s[2 * i], t.s[2 * i + 1]);
+      c0[i] = mul2(c, w.v[i]), s0[i] = mul2(s, w.v[i]);
+      c1[i] = mul2(c, w.v[kE / 2 + i]);
+      s1[i] = mul2(pack2(-t.s[2 * i], -t.s[2 * i + 1]), w.v[kE / 2 + i]);
     }
   }
-  const int64_t pos = position_of(p, t);
-  const bool inside = pos >= 0 && pos < p.table_rows;
-  float c[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f}, w[8];
-  if (inside && m.rotated) load_angles(p.table + pos * p.rotary, p.rotary, l, c, sn);
-  if (m.active) load_weights<INTER>(s.w, p.w_dtype, m, w);
-  T* out = static_cast<T*>(s.out) + (int64_t)t * s.heads * p.dim;
+};
+
+// y of one row.
+template <int LPR, bool INTER>
+__device__ __forceinline__ void fwd_row(const Params& p, const LaneMap& m, const float (&f)[2 * kE], const Lane& w,
+                                        uint32_t t, int l, bool inside, const Turn& turn, float (&out)[2 * kE]) {
+  const Lane x = lane_of(f);
+  const float ss = row_sum<LPR>(dot_of(x, x));
+  const float r = inside ? rsqrtf(ss * p.inv_dim + p.eps) : nan_f32();
+  const F2 rr = twice(r);
+  Lane y;
 #pragma unroll
-  for (int i = 0; i < kRowsPerLane; ++i) {
-    float a[4], b[4], v[8], ss = 0.f;
-    unpack4(raw[i][0], a);
-    unpack4(raw[i][1], b);
-    to_pairs<INTER>(a, b, v);
+  for (int e = 0; e < kE / 2; ++e) {
+    y.v[e] = mul2(rr, fma2(x.v[e], turn.c0[e], mul2(x.v[kE / 2 + e], turn.s1[e])));
+    y.v[kE / 2 + e] = mul2(rr, fma2(x.v[kE / 2 + e], turn.c1[e], mul2(x.v[e], turn.s0[e])));
+  }
+  floats_of(y, out);
+  if (!(ss < INFINITY)) {  // an infinite or NaN row: element by element, as the formula has it
+    float g[2 * kE];
+    floats_of(w, g);
 #pragma unroll
-    for (int e = 0; e < 8; ++e) ss = fmaf(v[e], v[e], ss);
-    ss = row_sum<LPR>(ss);
-    const float r = inside ? rsqrtf(ss * p.inv_dim + p.eps) : nan_f32();
-    const int h = h0 + i * kSub;
-    if (h < s.heads && m.active) {
-#pragma unroll
-      for (int e = 0; e < 8; ++e) v[e] = v[e] * r * w[e];
-      if (m.rotated) rotate8(v, c, sn);
-      store8<INTER>(out + (int64_t)h * p.dim, m, v);
+    for (int e = 0; e < 2 * kE; ++e) out[e] = f[e] * r * g[e];
+    if (m.rotated) {
+      Positions positions;
+      Angles again;
+      again.load(p, positions, m, t, l);
+      rotate_lane(out, again.c, again.s);
     }
   }
 }
 
-// ------------------------------------------------------------------ backward
-template <typename T, int LPR, bool INTER>
-__global__ void __launch_bounds__(kWarps * 32) bwd_kernel(const __grid_constant__ Params p) {
-  constexpr int kSub = 32 / LPR;
-  __shared__ __align__(16) float sums[kWarps][kMaxDimFast];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LPR;
-  const LaneMap m = lane_map<INTER>(l, p.dim, p.rotary);
-  float dw[2][8], w[2][8];
+// dx of one row, and its part of dw.
+template <int LPR>
+__device__ __forceinline__ void bwd_row(const Params& p, const LaneMap& m, const Lane& x, const Lane& g,
+                                        const Lane& w, const Angles& t, bool counts, Lane& dw,
+                                        float (&out)[2 * kE]) {
+  // u = R^T g, the transposed rotation; part = u x element by element
+  Lane u = g, part;
+  if (m.rotated) {
 #pragma unroll
-  for (int e = 0; e < 8; ++e) dw[0][e] = dw[1][e] = 0.f, w[0][e] = w[1][e] = 0.f;
-  if (m.active) {
-    load_weights<INTER>(p.side[0].w, p.w_dtype, m, w[0]);
-    load_weights<INTER>(p.side[1].w, p.w_dtype, m, w[1]);
+    for (int e = 0; e < kE / 2; ++e) {
+      const F2 c = pack2(t.c[2 * e], t.c[2 * e + 1]), s = pack2(t.s[2 * e], t.s[2 * e + 1]),
+               minus = pack2(-t.s[2 * e], -t.s[2 * e + 1]);
+      u.v[e] = fma2(g.v[e], c, mul2(g.v[kE / 2 + e], s));
+      u.v[kE / 2 + e] = fma2(g.v[kE / 2 + e], c, mul2(g.v[e], minus));
+    }
   }
-  for (uint32_t unit = blockIdx.x * kWarps + warp; unit < p.units; unit += gridDim.x * kWarps) {
-    const uint32_t t = unit / p.chunks;
-    uint32_t chunk = unit - t * p.chunks;
-    const bool is_k = chunk >= p.q_chunks;
-    if (is_k) chunk -= p.q_chunks;
-    const Side& s = p.side[is_k];
-    const int h0 = chunk * (kSub * kRowsPerLaneB) + lane / LPR;
-    const T* x = static_cast<const T*>(s.x) + (int64_t)t * s.x_ts;
-    const T* g = static_cast<const T*>(s.g) + (int64_t)t * s.g_ts;
-    Raw4<T> rx[kRowsPerLaneB][2], rg[kRowsPerLaneB][2];
 #pragma unroll
-    for (int i = 0; i < kRowsPerLaneB; ++i) {
-      const int h = h0 + i * kSub;
-      if (h < s.heads && m.active) {
-        rx[i][0] = load4(x + h * s.x_hs + m.a);
-        rx[i][1] = load4(x + h * s.x_hs + m.b);
-        rg[i][0] = load4(g + h * s.g_hs + m.a);
-        rg[i][1] = load4(g + h * s.g_hs + m.b);
-      } else {
-        rx[i][0].u = rx[i][1].u = {};
-        rg[i][0].u = rg[i][1].u = {};
+  for (int e = 0; e < kE; ++e) part.v[e] = mul2(u.v[e], x.v[e]);
+  // mean(w u x') = r mean(w u x): both sums from the row as it was read
+  const float ss = row_sum<LPR>(dot_of(x, x)), dot = row_sum<LPR>(dot_of(part, w));
+  const float r = t.inside ? rsqrtf(ss * p.inv_dim + p.eps) : nan_f32();
+  const F2 rr = twice(r), minus_k = twice(-(dot * r * p.inv_dim * r * r));  // dx = r w u - k x
+  const F2 count = counts ? rr : twice(0.f);
+  Lane y;
+#pragma unroll
+  for (int e = 0; e < kE; ++e) {
+    if (counts) dw.v[e] = fma2(part.v[e], count, dw.v[e]);
+    y.v[e] = fma2(mul2(u.v[e], w.v[e]), rr, mul2(x.v[e], minus_k));
+  }
+  floats_of(y, out);
+}
+
+// The rows of a step: heads h, h + SUB, ... below `end`, each lane's two runs.
+template <typename T, int ROWS, int SUB>
+__device__ __forceinline__ void fetch(const T* row, int64_t hs, const LaneMap& m, int h, int end,
+                                      Raw<T> (&raw)[ROWS][2]) {
+#pragma unroll
+  for (int i = 0; i < ROWS; ++i) {
+    raw[i][0].u = raw[i][1].u = {};
+    if (m.active && h + i * SUB < end) {
+      raw[i][0] = load_run(row + m.a);
+      raw[i][1] = load_run(row + m.b);
+    }
+    row += SUB * hs;
+  }
+}
+
+template <typename T, int LPR, bool INTER>
+__global__ void __launch_bounds__(kWarps * 32, kResident<false>) fwd_kernel(const __grid_constant__ Params p) {
+  constexpr int kRows = kRowsOf<T, false>, kSub = 32 / LPR, kSlots = kSub * kRows;
+  const Side& s = p.side[blockIdx.x >= p.side[1].first_block];
+  const int lane = threadIdx.x & 31, l = lane % LPR, sub = lane / LPR;
+  const LaneMap m = lane_map<INTER>(l, p.dim, p.rotary);
+  const uint32_t first = (blockIdx.x - s.first_block) * kWarps + (threadIdx.x >> 5), stride = s.blocks * kWarps;
+  Lane w{};
+  if (m.active) w = weights_of<INTER>(s.w, p.w_dtype, m);
+  T* const out = static_cast<T*>(s.out);
+  Positions positions;
+  if (s.flat) {
+    const uint32_t rows = (uint32_t)p.tokens * s.heads;
+    for (uint32_t item = first; item < s.items; item += stride) {
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const uint32_t row = item * kSlots + i * kSub + sub, t = row / (uint32_t)s.heads;
+        const bool ok = row < rows && m.active;
+        Raw<T> raw[2];
+        raw[0].u = raw[1].u = {};
+        Angles angles;
+        if (ok) {
+          const T* x = static_cast<const T*>(s.x) + t * s.x_ts + (row - t * s.heads) * s.x_hs;
+          raw[0] = load_run(x + m.a), raw[1] = load_run(x + m.b);
+          angles.load(p, positions, m, t, l);
+        }
+        float f[2 * kE], y[2 * kE];
+        unpack_lane<INTER>(raw, f);
+        fwd_row<LPR, INTER>(p, m, f, w, t, l, angles.inside, Turn(angles, w), y);
+        if (ok) store_lane<INTER>(out + (int64_t)row * p.dim + m.a, out + (int64_t)row * p.dim + m.b, y);
       }
     }
-    const int64_t pos = position_of(p, t);
-    const bool inside = pos >= 0 && pos < p.table_rows;
-    float c[4] = {1.f, 1.f, 1.f, 1.f}, sn[4] = {0.f, 0.f, 0.f, 0.f};
-    if (inside && m.rotated) load_angles(p.table + pos * p.rotary, p.rotary, l, c, sn);
+    return;
+  }
+  for (uint32_t item = first; item < s.items; item += stride) {
+    const uint32_t t = item / s.spans, chunk = (item - t * s.spans) * s.span;
+    int h = (int)chunk * kSlots + sub;
+    const int end = min((int)(chunk + s.span) * kSlots, s.heads);
+    const T* x = static_cast<const T*>(s.x) + (int64_t)t * s.x_ts + h * s.x_hs;
+    T* to = out + ((int64_t)t * s.heads + h) * p.dim;
+    Raw<T> raw[kRows][2];
+    fetch<T, kRows, kSub>(x, s.x_hs, m, h, end, raw);
+    Angles angles;
+    angles.load(p, positions, m, t, l);
+    const Turn turn(angles, w);
+    const bool inside = angles.inside;
+    while (true) {
 #pragma unroll
-    for (int e = 0; e < 4; ++e) sn[e] = -sn[e];  // the transposed rotation
-#pragma unroll
-    for (int i = 0; i < kRowsPerLaneB; ++i) {
-      float a[4], b[4], v[8], u[8], ss = 0.f, dot = 0.f;
-      unpack4(rx[i][0], a);
-      unpack4(rx[i][1], b);
-      to_pairs<INTER>(a, b, v);
-      unpack4(rg[i][0], a);
-      unpack4(rg[i][1], b);
-      to_pairs<INTER>(a, b, u);
-      if (m.rotated) rotate8(u, c, sn);
-      // both sums in one round of shuffles: mean(u * x') = r mean(u * x)
-#pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        ss = fmaf(v[e], v[e], ss);
-        dot = fmaf(u[e] * (is_k ? w[1][e] : w[0][e]), v[e], dot);
+      for (int i = 0; i < kRows; ++i) {
+        float f[2 * kE], y[2 * kE];
+        unpack_lane<INTER>(raw[i], f);
+        fwd_row<LPR, INTER>(p, m, f, w, t, l, inside, turn, y);
+        if (h + i * kSub < end && m.active) store_lane<INTER>(to + m.a, to + m.b, y);
+        to += kSub * p.dim;
       }
-      ss = row_sum<LPR>(ss);
-      dot = row_sum<LPR>(dot);
-      const int h = h0 + i * kSub;
-      const bool mine = h < s.heads && m.active;
-      const float r = inside ? rsqrtf(ss * p.inv_dim + p.eps) : nan_f32();
-      const float mean = dot * r * p.inv_dim;
+      h += kSlots;
+      x += kSlots * s.x_hs;
+      if (h - sub >= end) break;
+      fetch<T, kRows, kSub>(x, s.x_hs, m, h, end, raw);
+    }
+  }
+}
+
+template <typename T, int LPR, bool INTER>
+__global__ void __launch_bounds__(kWarps * 32, kResident<true>) bwd_kernel(const __grid_constant__ Params p) {
+  constexpr int kRows = kRowsOf<T, true>, kSub = 32 / LPR, kSlots = kSub * kRows;
+  __shared__ __align__(16) float sums[kWarps][kMaxDimFast];
+  const Side& s = p.side[blockIdx.x >= p.side[1].first_block];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LPR, sub = lane / LPR;
+  const LaneMap m = lane_map<INTER>(l, p.dim, p.rotary);
+  const uint32_t first = (blockIdx.x - s.first_block) * kWarps + warp, stride = s.blocks * kWarps;
+  Lane w{}, dw{};
+  if (m.active) w = weights_of<INTER>(s.w, p.w_dtype, m);
+  T* const out = static_cast<T*>(s.out);
+  Positions positions;
+  if (s.flat) {
+    const uint32_t rows = (uint32_t)p.tokens * s.heads;
+    for (uint32_t item = first; item < s.items; item += stride) {
 #pragma unroll
-      for (int e = 0; e < 8; ++e) {
-        const float hat = v[e] * r;
-        // rows past the last head count nothing (their r is eps^-1/2, or NaN)
-        const float part = mine ? u[e] * hat : 0.f;
-        if (is_k) dw[1][e] += part; else dw[0][e] += part;
-        v[e] = r * (u[e] * (is_k ? w[1][e] : w[0][e]) - hat * mean);
+      for (int i = 0; i < kRows; ++i) {
+        const uint32_t row = item * kSlots + i * kSub + sub, t = row / (uint32_t)s.heads;
+        const bool ok = row < rows && m.active;
+        Raw<T> rx[2], rg[2];
+        rx[0].u = rx[1].u = rg[0].u = rg[1].u = {};
+        Angles angles;
+        if (ok) {
+          const uint32_t h = row - t * s.heads;
+          const T* x = static_cast<const T*>(s.x) + t * s.x_ts + h * s.x_hs;
+          const T* g = static_cast<const T*>(s.g) + t * s.g_ts + h * s.g_hs;
+          rx[0] = load_run(x + m.a), rx[1] = load_run(x + m.b);
+          rg[0] = load_run(g + m.a), rg[1] = load_run(g + m.b);
+          angles.load(p, positions, m, t, l);
+        }
+        float fx[2 * kE], fg[2 * kE], y[2 * kE];
+        unpack_lane<INTER>(rx, fx);
+        unpack_lane<INTER>(rg, fg);
+        bwd_row<LPR>(p, m, lane_of(fx), lane_of(fg), w, angles, ok, dw, y);
+        if (ok && out) store_lane<INTER>(out + (int64_t)row * p.dim + m.a, out + (int64_t)row * p.dim + m.b, y);
       }
-      if (mine && s.out) store8<INTER>(static_cast<T*>(s.out) + ((int64_t)t * s.heads + h) * p.dim, m, v);
+    }
+  } else {
+    for (uint32_t item = first; item < s.items; item += stride) {
+      const uint32_t t = item / s.spans, chunk = (item - t * s.spans) * s.span;
+      int h = (int)chunk * kSlots + sub;
+      const int end = min((int)(chunk + s.span) * kSlots, s.heads);
+      const T* x = static_cast<const T*>(s.x) + (int64_t)t * s.x_ts + h * s.x_hs;
+      const T* g = static_cast<const T*>(s.g) + (int64_t)t * s.g_ts + h * s.g_hs;
+      int64_t to = ((int64_t)t * s.heads + h) * p.dim;
+      Raw<T> rx[kRows][2], rg[kRows][2];
+      fetch<T, kRows, kSub>(x, s.x_hs, m, h, end, rx);
+      fetch<T, kRows, kSub>(g, s.g_hs, m, h, end, rg);
+      Angles angles;
+      angles.load(p, positions, m, t, l);
+      while (true) {
+#pragma unroll
+        for (int i = 0; i < kRows; ++i) {
+          float fx[2 * kE], fg[2 * kE], y[2 * kE];
+          unpack_lane<INTER>(rx[i], fx);
+          unpack_lane<INTER>(rg[i], fg);
+          const bool ok = h + i * kSub < end && m.active;
+          bwd_row<LPR>(p, m, lane_of(fx), lane_of(fg), w, angles, ok, dw, y);
+          if (ok && out) store_lane<INTER>(out + to + m.a, out + to + m.b, y);
+          to += kSub * p.dim;
+        }
+        h += kSlots;
+        x += kSlots * s.x_hs;
+        g += kSlots * s.g_hs;
+        if (h - sub >= end) break;
+        fetch<T, kRows, kSub>(x, s.x_hs, m, h, end, rx);
+        fetch<T, kRows, kSub>(g, s.g_hs, m, h, end, rg);
+      }
     }
   }
   if (!p.partial) return;
+  float sum[2 * kE];
+  floats_of(dw, sum);
 #pragma unroll
-  for (int side = 0; side < 2; ++side) {
+  for (int e = 0; e < 2 * kE; ++e) {
 #pragma unroll
-    for (int e = 0; e < 8; ++e) {
+    for (int o = LPR; o < 32; o <<= 1) sum[e] += __shfl_xor_sync(0xffffffffu, sum[e], o);
+  }
+  if (lane < LPR && m.active) {
+    float a[kE], b[kE];
+    from_pairs<INTER>(sum, a, b);
 #pragma unroll
-      for (int o = LPR; o < 32; o <<= 1) dw[side][e] += __shfl_xor_sync(0xffffffffu, dw[side][e], o);
-    }
-    if (lane < LPR && m.active) store8<INTER>(&sums[warp][0], m, dw[side]);
-    __syncthreads();
-    for (int d = threadIdx.x; d < p.dim; d += kWarps * 32) {
-      float acc = 0.f;
+    for (int e = 0; e < kE; ++e) sums[warp][m.a + e] = a[e], sums[warp][m.b + e] = b[e];
+  }
+  __syncthreads();
+  for (int d = threadIdx.x; d < p.dim; d += kWarps * 32) {
+    float acc = 0.f;
 #pragma unroll
-      for (int k = 0; k < kWarps; ++k) acc += sums[k][d];
-      p.partial[((int64_t)blockIdx.x * 2 + side) * p.dim + d] = acc;
-    }
-    __syncthreads();
+    for (int k = 0; k < kWarps; ++k) acc += sums[k][d];
+    p.partial[(int64_t)blockIdx.x * p.dim + d] = acc;
   }
 }
 
@@ -239,6 +374,7 @@ __global__ void __launch_bounds__(kWarps * 32) any_kernel(const __grid_constant_
   const Side& s = p.side[blockIdx.y];
   const int n_units = p.dim - p.rotary / 2;
   const int64_t rows = p.tokens * s.heads;
+  Positions positions;
   float dw[NU][2];
 #pragma unroll
   for (int j = 0; j < NU; ++j) dw[j][0] = dw[j][1] = 0.f;
@@ -247,7 +383,7 @@ __global__ void __launch_bounds__(kWarps * 32) any_kernel(const __grid_constant_
     const int h = (int)(row - t * s.heads);
     const T* x = static_cast<const T*>(s.x) + t * s.x_ts + h * s.x_hs;
     const T* g = BWD ? static_cast<const T*>(s.g) + t * s.g_ts + h * s.g_hs : nullptr;
-    const int64_t pos = position_of(p, t);
+    const int64_t pos = positions.of(p, t);
     const bool inside = pos >= 0 && pos < p.table_rows;
     const float* angles = p.table + (inside ? pos : 0) * p.rotary;
     float v[NU][2], u[BWD ? NU : 1][2], ss = 0.f, dot = 0.f;
@@ -320,23 +456,31 @@ __global__ void __launch_bounds__(kWarps * 32) any_kernel(const __grid_constant_
 }
 
 // ------------------------------------------------------------------ weight gradients
-// 32 columns a block, its 8 warps over the blocks' partial sums; float64 from here on
-// (a few hundred terms a column, free beside the reads).
-__global__ void __launch_bounds__(kWarps * 32)
-dw_kernel(const float* __restrict__ partial, int blocks, int dim, int w_dtype, void* __restrict__ dwq,
-          void* __restrict__ dwk) {
-  __shared__ double sums[kWarps][32];
-  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31;
-  const int d = blockIdx.x * 32 + lane, side = blockIdx.y;
-  void* dst = side ? dwk : dwq;
+// 32 columns a block, its 32 warps over the blocks' partial sums; float64 from here on (a few hundred terms
+// a column, free beside the reads). Row r of a side is partial[(first + r * step) * dim].
+struct PartialRows {
+  int first, rows, step;
+};
+constexpr int kDwWarps = 32;
+__global__ void __launch_bounds__(kDwWarps * 32)
+dw_kernel(const float* __restrict__ partial, PartialRows q_rows, PartialRows k_rows, int dim, int w_dtype,
+          void* __restrict__ dwq, void* __restrict__ dwk) {
+  __shared__ double sums[kDwWarps][32];
+  const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, d = blockIdx.x * 32 + lane;
+  const PartialRows at = blockIdx.y ? k_rows : q_rows;
+  void* dst = blockIdx.y ? dwk : dwq;
   if (!dst) return;
   double acc = 0.0;
-  if (d < dim)
-    for (int b = warp; b < blocks; b += kWarps) acc += (double)partial[((int64_t)b * 2 + side) * dim + d];
+  if (d < dim) {
+#pragma unroll 8
+    for (int r = warp; r < at.rows; r += kDwWarps)
+      acc += (double)partial[((int64_t)at.first + (int64_t)r * at.step) * dim + d];
+  }
   sums[warp][lane] = acc;
   __syncthreads();
   if (warp != 0 || d >= dim) return;
-  for (int k = 1; k < kWarps; ++k) acc += sums[k][lane];
+#pragma unroll
+  for (int k = 1; k < kDwWarps; ++k) acc += sums[k][lane];
   const float f = (float)acc;
   if (w_dtype == MSA_F32) reinterpret_cast<float*>(dst)[d] = f;
   else if (w_dtype == MSA_F16) reinterpret_cast<__half*>(dst)[d] = __float2half_rn(f);
@@ -344,28 +488,52 @@ dw_kernel(const float* __restrict__ partial, int blocks, int dim, int w_dtype, v
 }
 
 // ------------------------------------------------------------------ host
-int lanes_per_row(int dim) { return dim <= 32 ? 4 : dim <= 64 ? 8 : dim <= 128 ? 16 : 32; }
-
-bool fast_shape(const Params& p, int dtype, bool bwd) {
-  const int es = elem_size(dtype);
-  if (p.dim % 8 || p.rotary % 8 || p.dim > kMaxDimFast || reinterpret_cast<uintptr_t>(p.table) % 16) return false;
+// Whether every row can be taken in runs of four elements.
+bool runs_fit(const Params& p, int es, bool bwd) {
+  if (p.dim % (2 * kE) || p.rotary % (2 * kE) || p.dim > kMaxDimFast || reinterpret_cast<uintptr_t>(p.table) % 16)
+    return false;
   for (const Side& s : p.side) {
-    if (!rows_aligned(s.x, s.x_ts, s.x_hs, es) || !rows_aligned(s.out, 0, 0, es)) return false;
-    if (bwd && !rows_aligned(s.g, s.g_ts, s.g_hs, es)) return false;
+    if (!rows_aligned(s.x, s.x_ts, s.x_hs, es, kE * es) || !rows_aligned(s.out, 0, 0, es, kE * es)) return false;
+    if (bwd && !rows_aligned(s.g, s.g_ts, s.g_hs, es, kE * es)) return false;
+    if (p.tokens * s.heads >= (int64_t)1 << 31) return false;  // 32-bit row numbers
   }
   return true;
 }
 
-// Blocks of the backward (and rows of its partial sums): enough for the chip, no more
-// than there is work.
-constexpr int kBwdBlocks = 148 * 6;
-int bwd_blocks(int64_t units) {
-  return (int)std::max<int64_t>(1, std::min<int64_t>(kBwdBlocks, (units + kWarps - 1) / kWarps));
+// The blocks of a launch stay on the chip; the backward's number bounds the rows of its partial sums (the
+// any-shape kernel has as many for each side).
+template <bool BWD>
+constexpr int kMaxBlocks = 148 * kResident<BWD>;
+int blocks_for(int64_t items, int most) {
+  return (int)std::max<int64_t>(1, std::min<int64_t>(most, (items + kWarps - 1) / kWarps));
 }
 
-template <typename T, int LPR>
-void launch_fast(const Params& p, bool bwd, int blocks, cudaStream_t st) {
-  if (bwd) {
+// Items of both sides, and each side's share of the blocks.
+int deal(Params& p, int slots, int most) {
+  int64_t steps[2];
+  for (int i = 0; i < 2; ++i) {
+    Side& s = p.side[i];
+    s.flat = s.heads < slots;
+    s.chunks = ceil_div(s.heads, slots);
+    steps[i] = s.flat ? ceil_div(p.tokens * s.heads, slots) : p.tokens * s.chunks;
+    // as many steps to an item as leave every warp eight items or more
+    s.span = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(s.chunks, steps[i] / ((int64_t)most * kWarps * 8)));
+    s.spans = ceil_div(s.chunks, s.span);
+    s.items = (uint32_t)(s.flat ? steps[i] : p.tokens * s.spans);
+  }
+  int k_blocks = (int)std::max<int64_t>(1, (most * steps[1] + (steps[0] + steps[1]) / 2) / (steps[0] + steps[1]));
+  k_blocks = std::min(blocks_for(p.side[1].items, most - 1), k_blocks);
+  p.side[0].first_block = 0;
+  p.side[0].blocks = blocks_for(p.side[0].items, most - k_blocks);
+  p.side[1].first_block = p.side[0].blocks;
+  p.side[1].blocks = k_blocks;
+  return p.side[0].blocks + k_blocks;
+}
+
+template <typename T, int LPR, bool BWD>
+void launch_rows(Params& p, cudaStream_t st) {
+  const int blocks = deal(p, 32 / LPR * kRowsOf<T, BWD>, kMaxBlocks<BWD>);
+  if constexpr (BWD) {
     if (p.interleaved) bwd_kernel<T, LPR, true><<<blocks, kWarps * 32, 0, st>>>(p);
     else bwd_kernel<T, LPR, false><<<blocks, kWarps * 32, 0, st>>>(p);
   } else {
@@ -374,27 +542,27 @@ void launch_fast(const Params& p, bool bwd, int blocks, cudaStream_t st) {
   }
 }
 
+template <typename T, bool BWD>
+void launch_runs(Params& p, cudaStream_t st) {
+  const int lanes = p.dim / (2 * kE);
+  if (lanes <= 4) launch_rows<T, 4, BWD>(p, st);
+  else if (lanes <= 8) launch_rows<T, 8, BWD>(p, st);
+  else if (lanes <= 16) launch_rows<T, 16, BWD>(p, st);
+  else launch_rows<T, 32, BWD>(p, st);
+}
+
 template <typename T>
 int launch(Params p, int dtype, bool bwd, void* dwq, void* dwk, cudaStream_t st) {
-  int blocks;
-  if (fast_shape(p, dtype, bwd)) {
-    const int lpr = lanes_per_row(p.dim);
-    const int rows = 32 / lpr * (bwd ? kRowsPerLaneB : kRowsPerLane);
-    p.q_chunks = ceil_div(p.side[0].heads, rows);
-    p.chunks = p.q_chunks + ceil_div(p.side[1].heads, rows);
-    const int64_t units = p.tokens * p.chunks;
-    MSA_CHECK_ARG(units < (int64_t)1 << 31, "msa_qk_norm_rope: too many tokens * heads");
-    p.units = (uint32_t)units;
-    blocks = bwd ? bwd_blocks(units) : ceil_div(units, kWarps);
-    switch (lpr) {
-      case 4: launch_fast<T, 4>(p, bwd, blocks, st); break;
-      case 8: launch_fast<T, 8>(p, bwd, blocks, st); break;
-      case 16: launch_fast<T, 16>(p, bwd, blocks, st); break;
-      default: launch_fast<T, 32>(p, bwd, blocks, st); break;
-    }
+  PartialRows q_rows, k_rows;
+  if (runs_fit(p, elem_size(dtype), bwd)) {
+    if (bwd) launch_runs<T, true>(p, st);
+    else launch_runs<T, false>(p, st);
+    q_rows = PartialRows{0, (int)p.side[0].blocks, 1};
+    k_rows = PartialRows{(int)p.side[1].first_block, (int)p.side[1].blocks, 1};
   } else {
     const bool small = p.dim - p.rotary / 2 <= 128;
-    blocks = bwd_blocks(p.tokens * std::max(p.side[0].heads, p.side[1].heads));
+    const int blocks = blocks_for(p.tokens * std::max(p.side[0].heads, p.side[1].heads),
+                                  bwd ? kMaxBlocks<true> : kMaxBlocks<false>);
     const dim3 grid(blocks, 2);
     if (bwd) {
       if (small) any_kernel<T, 4, true><<<grid, kWarps * 32, 0, st>>>(p);
@@ -403,11 +571,14 @@ int launch(Params p, int dtype, bool bwd, void* dwq, void* dwk, cudaStream_t st)
       if (small) any_kernel<T, 4, false><<<grid, kWarps * 32, 0, st>>>(p);
       else any_kernel<T, 16, false><<<grid, kWarps * 32, 0, st>>>(p);
     }
+    q_rows = PartialRows{0, blocks, 2};
+    k_rows = PartialRows{1, blocks, 2};
   }
   count_launches(1);
   if (int e = launch_status("qk_norm_rope")) return e;
   if (bwd && p.partial) {
-    dw_kernel<<<dim3(ceil_div(p.dim, 32), 2), kWarps * 32, 0, st>>>(p.partial, blocks, p.dim, p.w_dtype, dwq, dwk);
+    dw_kernel<<<dim3(ceil_div(p.dim, 32), 2), kDwWarps * 32, 0, st>>>(p.partial, q_rows, k_rows, p.dim, p.w_dtype,
+                                                                      dwq, dwk);
     count_launches(1);
     return launch_status("qk_norm_rope dw");
   }
@@ -457,7 +628,7 @@ extern "C" int msa_qk_norm_rope_fwd(const void* q, const void* k, int dtype, con
 }
 
 extern "C" size_t msa_qk_norm_rope_bwd_workspace_size(int32_t head_dim) {
-  return sizeof(float) * 2 * (size_t)kBwdBlocks * head_dim;
+  return sizeof(float) * 2 * (size_t)kMaxBlocks<true> * head_dim;
 }
 
 extern "C" int msa_qk_norm_rope_bwd(const void* q, const void* k, const void* grad_q, const void* grad_k, int dtype,

@@ -25,7 +25,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import DTYPE_CODE, call, ptr, stream_of
+from ._lib import DTYPE_CODE, call, device_of, ptr, stream_of
 
 
 def _check_paged(block_table, seq_lens, batch, device):
@@ -156,12 +156,12 @@ def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, blo
 def _sparse_decode8(q, k_cache, v_cache, block_table, seq_lens, indices, block_size, scale, return_lse, k_scale,
                     v_scale):
     batch, hq, dim = q.shape
-    out = torch.empty((batch, hq, dim), dtype=q.dtype, device=q.device)
-    lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device)
+    out = q.new_empty(q.shape)
+    lse = q.new_empty((batch, hq), dtype=torch.float32)
     if batch and dim:
         dense = [x if x.shape[3] == 1 or x.stride(3) == 1 else x.contiguous() for x in (k_cache, v_cache)]
         qc, table, lens, ids = q.contiguous(), block_table.contiguous(), seq_lens.contiguous(), indices.contiguous()
-        with torch.cuda.device(q.device):
+        with device_of(q):
             call("msa_decode_attn_e4m3", ptr(qc), DTYPE_CODE[q.dtype], ptr(dense[0]), ptr(dense[1]),
                  *dense[0].stride()[:3], *dense[1].stride()[:3], ptr(k_scale), ptr(v_scale), ptr(table), ptr(lens),
                  ptr(ids), batch, hq, k_cache.shape[2], dim, k_cache.shape[1], table.shape[1], k_cache.shape[0],

@@ -23,7 +23,7 @@ import math
 import torch
 
 from . import _lib
-from ._lib import DTYPE_CODE, call, ptr, stream_of
+from ._lib import DTYPE_CODE, call, device_of, ptr, stream_of
 from .layout import sequence_lengths
 
 MAX_HEAD_DIM = 512
@@ -77,9 +77,8 @@ def _laid_out(q, k, q_weight, k_weight, table, positions, cu):
 def norm_rope_forward(q, k, q_weight, k_weight, table, positions, cu, eps, interleaved):
     """(q_out, k_out); shared by the autograd Function and the torch.library operator."""
     q, k, q_weight, k_weight, table, positions, cu = _laid_out(q, k, q_weight, k_weight, table, positions, cu)
-    q_out = torch.empty(q.shape, dtype=q.dtype, device=q.device)
-    k_out = torch.empty(k.shape, dtype=k.dtype, device=k.device)
-    with torch.cuda.device(q.device):
+    q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+    with device_of(q):
         call("msa_qk_norm_rope_fwd", ptr(q), ptr(k), *_common(q, k, q_weight, k_weight, table, positions, cu,
                                                               interleaved),
              float(eps), ptr(q_out), ptr(k_out), stream_of(q))
@@ -92,11 +91,10 @@ def norm_rope_backward(q, k, q_weight, k_weight, table, positions, cu, eps, inte
         return None, None, None, None
     q, k, q_weight, k_weight, table, positions, cu = _laid_out(q, k, q_weight, k_weight, table, positions, cu)
     gq, gk = dense_rows(grad_q.to(q.dtype)), dense_rows(grad_k.to(k.dtype))
-    dq, dk, dwq, dwk = (torch.empty(x.shape, dtype=x.dtype, device=x.device) if n else None
-                        for x, n in zip((q, k, q_weight, k_weight), need))
+    dq, dk, dwq, dwk = (x.new_empty(x.shape) if n else None for x, n in zip((q, k, q_weight, k_weight), need))
     ws_bytes = _lib.load().msa_qk_norm_rope_bwd_workspace_size(q.shape[2]) if need[2] or need[3] else 0
-    workspace = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
-    with torch.cuda.device(q.device):
+    workspace = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
+    with device_of(q):
         call("msa_qk_norm_rope_bwd", ptr(q), ptr(k), ptr(gq), ptr(gk),
              *_common(q, k, q_weight, k_weight, table, positions, cu, interleaved), gq.stride(0), gq.stride(1),
              gk.stride(0), gk.stride(1), float(eps), ptr(dq), ptr(dk), ptr(dwq), ptr(dwk), ptr(workspace), ws_bytes,
@@ -176,4 +174,6 @@ def m3_qk_norm_rope(
         from . import library
 
         return library.qk_norm_rope(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, interleaved)
+    if not (torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, q_weight, k_weight))):
+        return norm_rope_forward(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, interleaved)
     return _QKNormRope.apply(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, bool(interleaved))
