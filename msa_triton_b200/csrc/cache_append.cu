@@ -27,7 +27,11 @@ using namespace rope;
 
 constexpr int kWarps = 8;
 constexpr int kRowsPerLane = 4;
-constexpr int kKeep = 8;  // rows of a page that a lane holds in registers between the two passes
+constexpr int kPageWarps = 8;
+// Blocks to an SM: 3 with a few spilled registers 75 us at 32768 tokens of 8 heads of 128, 2 without 87 us.
+constexpr int kPageBlocks = 3;
+template <typename T>
+constexpr int kKeep = sizeof(T) == 4 ? 4 : 8;  // rows of a page that a lane holds between the two passes
 constexpr int kMaxDimFast = 256;
 
 struct Half {  // k or v
@@ -44,6 +48,7 @@ struct Params {
   const int32_t *cu, *block_table, *seq_lens;
   int64_t table_rows, tokens, num_pages;
   int batch, heads, dim, page_size, max_pages;
+  FastDiv by_page, by_page_parts;  // page_size; items of a page
   uint32_t units, chunks, head_chunks;
   bool interleaved;
 };
@@ -56,26 +61,28 @@ __device__ __forceinline__ int request_of(const Params& p, int64_t t) {
 }
 
 // Physical page of request b's logical page, or -1.
-__device__ __forceinline__ int64_t physical_page(const Params& p, int b, int64_t logical) {
+__device__ __forceinline__ int64_t physical_page(const Params& p, int b, int logical) {
   if (logical < 0 || logical >= p.max_pages) return -1;
   const int page = p.block_table[(int64_t)b * p.max_pages + logical];
   return page >= 0 && page < p.num_pages ? page : -1;
 }
 
-// New tokens of request b: rows [first, first + n), positions [pos, pos + n).
+// New tokens of request b: rows [first, first + n), positions [pos, pos + n). Lengths and boundaries are 32-bit;
+// what a broken cu_seqlens could overflow is 64.
 struct Span {
-  int64_t first, pos, n;
+  int64_t first;
+  int pos, n;
 };
 __device__ __forceinline__ Span span_of(const Params& p, int b) {
+  const int64_t begin = p.cu ? p.cu[b] : b, behind = p.cu ? p.cu[b + 1] : (int64_t)b + 1;
+  int64_t first = begin, pos = (int64_t)p.seq_lens[b] - (behind - begin);
+  if (pos < 0) first -= pos, pos = 0;  // tokens before position 0 are not stored
+  if (first < 0) pos -= first, first = 0;
+  const int64_t n = min(behind, p.tokens) - first;
   Span s;
-  s.first = p.cu ? p.cu[b] : b;
-  const int64_t end = p.cu ? min((int64_t)p.cu[b + 1], p.tokens) : (int64_t)b + 1;
-  const int64_t len = p.seq_lens[b];
-  s.n = p.cu ? (int64_t)p.cu[b + 1] - s.first : 1;
-  s.pos = len - s.n;
-  if (s.pos < 0) s.first -= s.pos, s.pos = 0;  // tokens before position 0 are not stored
-  if (s.first < 0) s.pos -= s.first, s.first = 0;
-  s.n = end - s.first;
+  s.first = first;
+  s.pos = (int)pos;
+  s.n = n > 0 && pos + n <= 0x7fffffff ? (int)n : 0;
   return s;
 }
 
@@ -105,14 +112,15 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
   }
   const int b = request_of(p, t);
   if (b < 0) return;
-  const int64_t pos = (int64_t)p.seq_lens[b] - (p.cu ? (int64_t)p.cu[b + 1] - t : 1);
-  if (pos < 0) return;
-  const int64_t page = physical_page(p, b, pos / p.page_size);
+  const int64_t pos64 = (int64_t)p.seq_lens[b] - (p.cu ? (int64_t)p.cu[b + 1] - t : 1);
+  if (pos64 < 0 || pos64 > 0x7fffffff) return;
+  const int pos = (int)pos64, logical = p.by_page(pos);
+  const int64_t page = physical_page(p, b, logical);
   if (page < 0) return;
   const bool rotated = m.rotated && s.rotary > 0, inside = s.rotary == 0 || pos < p.table_rows;
   float c[4], sn[4];
-  if (inside && rotated) load_angles(p.table + pos * s.rotary, s.rotary, l, c, sn);
-  T* out = static_cast<T*>(s.cache) + page * s.c_ps + (pos % p.page_size) * s.c_ts;
+  if (inside && rotated) load_angles(p.table + (int64_t)pos * s.rotary, s.rotary, l, c, sn);
+  T* out = static_cast<T*>(s.cache) + page * s.c_ps + (int64_t)(pos - logical * p.page_size) * s.c_ts;
 #pragma unroll
   for (int i = 0; i < kRowsPerLane; ++i) {
     const int h = h0 + i * kSub;
@@ -134,33 +142,37 @@ __global__ void __launch_bounds__(kWarps * 32) append_kernel(const __grid_consta
 // start at cu[b] / S + 2 b: at least as many lie between two requests as the pages that n tokens can
 // touch (n / S + 2), so a task finds its request by bisection without a scan over the requests.
 struct Task {
-  int64_t page, row_first, n, token, pos;  // physical page; first row in it; rows; k/v row; position
+  int64_t token;                     // row of k / v
+  int b, logical, row_first, n, pos;  // request, logical page, first row in it, rows, position of the first
 };
-__device__ __forceinline__ bool find_task(const Params& p, int64_t task, Task& r) {
-  int b;
-  int64_t index = 0;
-  if (!p.cu) {
-    b = (int)task;
-  } else {
+// False: nothing to do. The physical page is looked up apart (its loads would hold up the rows').
+__device__ __forceinline__ bool find_task(const Params& p, int task, Task& r) {
+  int b = task, index = 0;
+  if (p.cu) {
+    auto first_of = [&](int i) { return (int64_t)p.by_page(max(p.cu[i], 0)) + 2 * (int64_t)i; };
     int lo = 0, hi = p.batch - 1;
     while (lo < hi) {
       const int mid = (lo + hi + 1) >> 1;
-      if ((int64_t)p.cu[mid] / p.page_size + 2 * (int64_t)mid <= task) lo = mid; else hi = mid - 1;
+      if (first_of(mid) <= task) lo = mid; else hi = mid - 1;
     }
     b = lo;
-    index = task - ((int64_t)p.cu[b] / p.page_size + 2 * (int64_t)b);
+    const int64_t i = task - first_of(b);
+    if (i < 0 || i >= p.max_pages) return false;
+    index = (int)i;
   }
   const Span s = span_of(p, b);
-  if (index < 0 || s.n <= 0) return false;
-  const int64_t logical = s.pos / p.page_size + index;
-  const int64_t lo = max(s.pos, logical * p.page_size), hi = min(s.pos + s.n, (logical + 1) * p.page_size);
+  if (s.n <= 0) return false;
+  const int logical = p.by_page(s.pos) + index;
+  const int64_t page_begin = (int64_t)logical * p.page_size;
+  const int64_t lo = max((int64_t)s.pos, page_begin), hi = min((int64_t)s.pos + s.n, page_begin + p.page_size);
   if (lo >= hi) return false;
-  r.page = physical_page(p, b, logical);
-  r.row_first = lo - logical * p.page_size;
-  r.n = hi - lo;
-  r.pos = lo;
+  r.b = b;
+  r.logical = logical;
+  r.row_first = (int)(lo - page_begin);
+  r.n = (int)(hi - lo);
+  r.pos = (int)lo;
   r.token = s.first + (lo - s.pos);
-  return r.page >= 0;
+  return true;
 }
 
 // Earlier rows of the page to the new scale, 16 codes a thread and step.
@@ -178,7 +190,7 @@ __device__ __forceinline__ void move_rows(uint8_t* page, int64_t row_stride, int
 }
 
 // New scale of the page, given its new rows' maximum.
-__device__ __forceinline__ float grown_scale(float amax, int64_t row_first, float old) {
+__device__ __forceinline__ float grown_scale(float amax, int row_first, float old) {
   const float need = e4m3::scale_for(amax);
   return row_first == 0 ? need : fmaxf(old, need);
 }
@@ -214,7 +226,7 @@ __device__ __forceinline__ void rotated_row(const Params& p, const Half& s, cons
     for (int j = 0; j < 8; ++j) v[j] = nan_f32();
   } else if (m.rotated) {
     float c[4], sn[4];
-    load_angles(p.table + pos * s.rotary, s.rotary, l, c, sn);
+    load_angles(p.table + (int64_t)pos * s.rotary, s.rotary, l, c, sn);
     rotate_lane(v, c, sn);
   }
 }
@@ -234,8 +246,10 @@ __global__ void __launch_bounds__(kWarps * 32) append8_token_kernel(const __grid
   Raw<T> raw[2] = {};
   if (mine) raw[0] = load_run(x + m.a), raw[1] = load_run(x + m.b);
   Task t;
-  if (!find_task(p, b, t)) return;
-  float* scale = s.scale + t.page * p.heads + h;
+  if (!find_task(p, (int)b, t)) return;
+  const int64_t at = physical_page(p, t.b, t.logical);
+  if (at < 0) return;
+  float* scale = s.scale + at * p.heads + h;
   const float old = *scale;
   float v[8], amax = 0.f;
   rotated_row<T, INTER>(p, s, m, l, raw, t.pos, v);
@@ -243,12 +257,18 @@ __global__ void __launch_bounds__(kWarps * 32) append8_token_kernel(const __grid
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) amax = fmaxf(amax, __shfl_xor_sync(0xffffffffu, amax, o));
   const float now = grown_scale(amax, t.row_first, old);
-  uint8_t* page = static_cast<uint8_t*>(s.cache) + t.page * s.c_ps + h * s.c_hs;
+  uint8_t* page = static_cast<uint8_t*>(s.cache) + at * s.c_ps + h * s.c_hs;
   if (mine) store_codes<INTER>(page + t.row_first * s.c_ts, m, v, 1.f / now);
   if (t.row_first > 0 && now > old) move_rows(page, s.c_ts, (int)t.row_first, p.dim, old / now, lane, 32);
   if (lane == 0 && now != old) *scale = now;
 }
 
+template <int BYTES>
+__device__ __forceinline__ void copy_run(uint32_t to, const void* from) {
+  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
+}
+
+template <int WARPS>
 __device__ __forceinline__ float block_amax(float v, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -256,70 +276,170 @@ __device__ __forceinline__ float block_amax(float v, float* red) {
   __syncthreads();
   v = red[0];
 #pragma unroll
-  for (int w = 1; w < kWarps; ++w) v = fmaxf(v, red[w]);
+  for (int w = 1; w < WARPS; ++w) v = fmaxf(v, red[w]);
   return v;
 }
 
-// Chunks: a block per (request, page, head) of k or v. The rows stay in registers between the pass
-// for the maximum and the pass that writes the codes (pages longer than kKeep rows a lane read the
-// rest again, from L2).
+// Chunks: an item of work is a (request, page, head) of k or v, the heads of a page one after the other (their
+// rows lie side by side in memory). Blocks stay and walk over the items. Every thread copies the runs of its
+// rows of the next item into places of its own in shared memory (cp.async: nothing to wait for but its own
+// copies), while it rotates the current ones into registers, takes the page's maximum and writes the codes. Rows past kKeep a
+// lane (pages longer than 128 rows of 128) are read twice from memory instead. The maximum takes whatever is
+// there: NaN drops out of fmaxf by itself, and only a page that holds an infinity is looked through again
+// for its finite values.
+// (Giving a block several heads of a page in a row keeps the angles in L1 but scatters the reads: 101 us
+// with four heads, 123 us with eight, at the sizes below.)
 template <typename T, int LPR, bool INTER>
-__global__ void __launch_bounds__(kWarps * 32) append8_page_kernel(const __grid_constant__ Params p) {
-  constexpr int kRows = kWarps * 32 / LPR;  // rows of a step
-  __shared__ float red[kWarps];
-  Task t;
-  if (!find_task(p, blockIdx.x, t)) return;  // the same for the whole block
-  const int h = blockIdx.y;
-  const Half& s = p.half[blockIdx.z];
-  const int l = threadIdx.x % LPR, r0 = threadIdx.x / LPR;
-  const LaneMap m = lane_map<INTER>(l, p.dim, s.rotary);
-  const T* x = static_cast<const T*>(s.x) + t.token * s.x_ts + h * s.x_hs;
-  float* scale = s.scale + t.page * p.heads + h;
-  const float old = *scale;
-  Raw<T> raw[kKeep][2];
+__global__ void __launch_bounds__(kPageWarps * 32, kPageBlocks) append8_page_kernel(const __grid_constant__ Params p) {
+  constexpr int kThreads = kPageWarps * 32, kRows = kThreads / LPR, kHeld = kKeep<T>, kRun = kE * (int)sizeof(T);
+  extern __shared__ __align__(16) uint8_t smem[];  // [2][kHeld][2][kThreads] runs
+  __shared__ float red[2][kPageWarps];
+  const int tid = threadIdx.x, l = tid % LPR, r0 = tid / LPR;
+  const uint32_t place = (uint32_t)__cvta_generic_to_shared(smem) + tid * kRun;
+
+  struct Item {
+    Task t;
+    int h;
+    bool is_v, some;
+  };
+  auto item_of = [&](uint32_t i) {
+    Item it;
+    it.some = i < p.units;
+    if (!it.some) return it;
+    const int task = p.by_page_parts((int)i), part = (int)i - task * (p.heads * (int)p.chunks);
+    it.is_v = part >= p.heads;
+    it.h = part - it.is_v * p.heads;
+    it.some = find_task(p, task, it.t);
+    return it;
+  };
+  auto issue = [&](const Item& it, int buffer) {
+    if (it.some) {
+      const Half& s = p.half[it.is_v];
+      const LaneMap m = lane_map<INTER>(l, p.dim, s.rotary);
+      const T* x = static_cast<const T*>(s.x) + (it.t.token + r0) * s.x_ts + it.h * s.x_hs + m.a;
+      const int n = m.active ? min(it.t.n, kHeld * kRows) : 0, d = m.b - m.a;
+      uint32_t to = place + buffer * (kHeld * 2 * kThreads * kRun);
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    const int r = r0 + i * kRows;
-    if (r < t.n && m.active) {
-      raw[i][0] = load_run(x + r * s.x_ts + m.a);
-      raw[i][1] = load_run(x + r * s.x_ts + m.b);
+      for (int i = 0; i < kHeld; ++i) {
+        if (r0 + i * kRows < n) {
+          copy_run<kRun>(to, x);
+          copy_run<kRun>(to + kThreads * kRun, x + d);
+        }
+        x += kRows * s.x_ts;
+        to += 2 * kThreads * kRun;
+      }
     }
-  }
-  float amax = 0.f, v[8];
+    asm volatile("cp.async.commit_group;" ::: "memory");
+  };
+
+  uint32_t index = blockIdx.x;
+  Item now = item_of(index);
+  issue(now, 0);
+  for (int turn = 0; index < p.units; turn ^= 1) {
+    index += gridDim.x;
+    const Item next = item_of(index);
+    issue(next, turn ^ 1);
+    asm volatile("cp.async.wait_group 1;" ::: "memory");
+    const Item it = now;
+    now = next;
+    if (!it.some) continue;  // the same for the whole block
+    const int64_t at = physical_page(p, it.t.b, it.t.logical);
+    if (at < 0) continue;
+    const Half& s = p.half[it.is_v];
+    const LaneMap m = lane_map<INTER>(l, p.dim, s.rotary);
+    float* scale = s.scale + at * p.heads + it.h;
+    const float old = *scale;
+    const int n = it.t.n, held = m.active ? min(n, kHeld * kRows) : 0;
+    const bool turned = m.rotated && s.rotary > 0;
+    // rows from here on have no angle
+    const int inside = s.rotary > 0 ? (int)min(max(p.table_rows - it.t.pos, (int64_t)0), (int64_t)n) : n;
+    const float* angles = turned ? p.table + (int64_t)(it.t.pos + r0) * s.rotary + kE * l : nullptr;
+    const uint8_t* mine = smem + tid * kRun + turn * (kHeld * 2 * kThreads * kRun);
+    auto turn_row = [&](Lane y, int r, const float* angle) {
+      if (r >= inside) {
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    const int r = r0 + i * kRows;
-    if (r < t.n && m.active) {
-      rotated_row<T, INTER>(p, s, m, l, raw[i], t.pos + r, v);
-      amax = amax8(v, amax);
-    }
-  }
-  for (int64_t r = r0 + kKeep * kRows; r < t.n; r += kRows) {
-    if (!m.active) continue;
-    const Raw<T> w[2] = {load_run(x + r * s.x_ts + m.a), load_run(x + r * s.x_ts + m.b)};
-    rotated_row<T, INTER>(p, s, m, l, w, t.pos + r, v);
-    amax = amax8(v, amax);
-  }
-  const float now = grown_scale(block_amax(amax, red), t.row_first, old), inv = 1.f / now;
-  uint8_t* page = static_cast<uint8_t*>(s.cache) + t.page * s.c_ps + h * s.c_hs;
-  uint8_t* out = page + t.row_first * s.c_ts;
+        for (int i = 0; i < kE; ++i) y.v[i] = twice(nan_f32());
+      } else if (turned) {
+        const float4 c = __ldg(reinterpret_cast<const float4*>(angle));
+        const float4 sn = __ldg(reinterpret_cast<const float4*>(angle + s.rotary / 2));
+        const float cc[kE] = {c.x, c.y, c.z, c.w}, ss[kE] = {sn.x, sn.y, sn.z, sn.w};
+        rotate_exact(y, cc, ss);
+      }
+      return y;
+    };
+    auto held_row = [&](int i) {
+      const Raw<T>* from = reinterpret_cast<const Raw<T>*>(mine + i * (2 * kThreads * kRun));
+      const Raw<T> raw[2] = {from[0], from[kThreads]};
+      float f[2 * kE];
+      unpack_lane<INTER>(raw, f);
+      return turn_row(lane_of(f), r0 + i * kRows, angles + i * (kRows * s.rotary));
+    };
+    auto reread = [&](int r) {
+      const T* x = static_cast<const T*>(s.x) + (it.t.token + r) * s.x_ts + it.h * s.x_hs;
+      const Raw<T> raw[2] = {load_run(x + m.a), load_run(x + m.b)};
+      float f[2 * kE];
+      unpack_lane<INTER>(raw, f);
+      return turn_row(lane_of(f), r, p.table + (int64_t)(it.t.pos + r) * s.rotary + kE * l);
+    };
+    // the largest magnitude, with or without the infinite ones
+    auto largest = [&](const Lane& v, float acc, bool finite) {
 #pragma unroll
-  for (int i = 0; i < kKeep; ++i) {
-    const int r = r0 + i * kRows;
-    if (r < t.n && m.active) {
-      rotated_row<T, INTER>(p, s, m, l, raw[i], t.pos + r, v);
-      store_codes<INTER>(out + r * s.c_ts, m, v, inv);
+      for (int i = 0; i < kE; ++i) {
+        const float2 f = unpack2(v.v[i]);
+        acc = fmaxf(acc, finite && !e4m3::finite(f.x) ? 0.f : fabsf(f.x));
+        acc = fmaxf(acc, finite && !e4m3::finite(f.y) ? 0.f : fabsf(f.y));
+      }
+      return acc;
+    };
+    Lane y[kHeld];
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i)
+      if (r0 + i * kRows < held) y[i] = held_row(i);
+      else y[i] = Lane{};
+    auto page_amax = [&](bool finite, float* red_at) {
+      float amax = 0.f;
+#pragma unroll
+      for (int i = 0; i < kHeld; ++i) amax = largest(y[i], amax, finite);
+      if (m.active)
+        for (int r = r0 + kHeld * kRows; r < n; r += kRows) amax = largest(reread(r), amax, finite);
+      return block_amax<kPageWarps>(amax, red_at);
+    };
+    float amax = page_amax(false, red[turn]);  // two places: the next item's are written before all have read these
+    const bool infinite = amax == INFINITY;
+    if (infinite) {
+      __syncthreads();
+      amax = page_amax(true, red[turn]);
     }
+    const float now_scale = grown_scale(amax, it.t.row_first, old), inv = 1.f / now_scale;
+    uint8_t* page = static_cast<uint8_t*>(s.cache) + at * s.c_ps + it.h * s.c_hs;
+    uint8_t* out = page + (it.t.row_first + r0) * s.c_ts;
+    auto put = [&](const Lane& v, uint8_t* to) {
+      float f[2 * kE], a[kE], b[kE];
+      if (infinite) {
+        floats_of(v, f);
+        store_codes<INTER>(to, m, f, inv);
+        return;
+      }
+      Lane z;
+#pragma unroll
+      for (int i = 0; i < kE; ++i) z.v[i] = mul2(v.v[i], twice(inv));
+      floats_of(z, f);
+      from_pairs<INTER>(f, a, b);
+      *reinterpret_cast<uint32_t*>(to + m.a) = e4m3::encode2(a[0], a[1]) | e4m3::encode2(a[2], a[3]) << 16;
+      *reinterpret_cast<uint32_t*>(to + m.b) = e4m3::encode2(b[0], b[1]) | e4m3::encode2(b[2], b[3]) << 16;
+    };
+#pragma unroll
+    for (int i = 0; i < kHeld; ++i) {
+      if (r0 + i * kRows < held) put(y[i], out);
+      out += kRows * s.c_ts;
+    }
+    if (m.active)
+      for (int64_t r = r0 + kHeld * kRows; r < n; r += kRows, out += kRows * s.c_ts) put(reread(r), out);
+    if (it.t.row_first > 0 && now_scale > old)
+      move_rows(page, s.c_ts, (int)it.t.row_first, p.dim, old / now_scale, tid, kThreads);
+    if (tid == 0 && now_scale != old) *scale = now_scale;
   }
-  for (int64_t r = r0 + kKeep * kRows; r < t.n; r += kRows) {
-    if (!m.active) continue;
-    const Raw<T> w[2] = {load_run(x + r * s.x_ts + m.a), load_run(x + r * s.x_ts + m.b)};
-    rotated_row<T, INTER>(p, s, m, l, w, t.pos + r, v);
-    store_codes<INTER>(out + r * s.c_ts, m, v, inv);
-  }
-  if (t.row_first > 0 && now > old)
-    move_rows(page, s.c_ts, (int)t.row_first, p.dim, old / now, threadIdx.x, kWarps * 32);
-  if (threadIdx.x == 0 && now != old) *scale = now;
+  asm volatile("cp.async.wait_group 0;" ::: "memory");
 }
 
 // ------------------------------------------------------------------ any shape
@@ -329,7 +449,9 @@ template <typename T>
 __global__ void __launch_bounds__(kWarps * 32) append_any_kernel(const __grid_constant__ Params p) {
   __shared__ float red[kWarps];
   Task t;
-  if (!find_task(p, blockIdx.x, t)) return;
+  if (!find_task(p, (int)blockIdx.x, t)) return;
+  const int64_t at = physical_page(p, t.b, t.logical);
+  if (at < 0) return;
   const int h = blockIdx.y;
   const Half& s = p.half[blockIdx.z];
   const int n_units = p.dim - s.rotary / 2;
@@ -353,7 +475,7 @@ __global__ void __launch_bounds__(kWarps * 32) append_any_kernel(const __grid_co
   Unit e;
   float a, b;
   if (!s.scale) {
-    T* page = static_cast<T*>(s.cache) + t.page * s.c_ps + h * s.c_hs;
+    T* page = static_cast<T*>(s.cache) + at * s.c_ps + h * s.c_hs;
     for (int64_t i = threadIdx.x; i < n; i += kWarps * 32) {
       value(i, row, e, a, b);
       T* out = page + (t.row_first + row) * s.c_ts;
@@ -362,15 +484,15 @@ __global__ void __launch_bounds__(kWarps * 32) append_any_kernel(const __grid_co
     }
     return;
   }
-  float* scale = s.scale + t.page * p.heads + h;
+  float* scale = s.scale + at * p.heads + h;
   const float old = *scale;
   float amax = 0.f;
   for (int64_t i = threadIdx.x; i < n; i += kWarps * 32) {
     value(i, row, e, a, b);
     amax = fmaxf(amax, fmaxf(e4m3::finite(a) ? fabsf(a) : 0.f, e4m3::finite(b) ? fabsf(b) : 0.f));
   }
-  const float now = grown_scale(block_amax(amax, red), t.row_first, old), inv = 1.f / now;
-  uint8_t* page = static_cast<uint8_t*>(s.cache) + t.page * s.c_ps + h * s.c_hs;
+  const float now = grown_scale(block_amax<kWarps>(amax, red), t.row_first, old), inv = 1.f / now;
+  uint8_t* page = static_cast<uint8_t*>(s.cache) + at * s.c_ps + h * s.c_hs;
   for (int64_t i = threadIdx.x; i < n; i += kWarps * 32) {
     value(i, row, e, a, b);
     uint8_t* out = page + (t.row_first + row) * s.c_ts;
@@ -379,8 +501,8 @@ __global__ void __launch_bounds__(kWarps * 32) append_any_kernel(const __grid_co
   }
   if (t.row_first > 0 && now > old)
     for (int64_t i = threadIdx.x; i < t.row_first * p.dim; i += kWarps * 32) {
-      uint8_t* at = page + (i / p.dim) * s.c_ts + i % p.dim;
-      *at = e4m3::encode1(e4m3::decode1(*at), old / now);
+      uint8_t* code = page + (i / p.dim) * s.c_ts + i % p.dim;
+      *code = e4m3::encode1(e4m3::decode1(*code), old / now);
     }
   if (threadIdx.x == 0 && now != old) *scale = now;
 }
@@ -403,22 +525,28 @@ bool fast_shape(const Params& p, int halves, int dtype, bool quantised) {
 }
 
 template <typename T, int LPR, bool INTER>
-void launch_fast(Params p, int halves, bool quantised, int64_t tasks, cudaStream_t st) {
+int launch_fast(Params p, int halves, bool quantised, int64_t tasks, cudaStream_t st) {
   if (!quantised) {
     append_kernel<T, LPR, INTER><<<ceil_div(p.units, kWarps), kWarps * 32, 0, st>>>(p);
   } else if (!p.cu) {
     append8_token_kernel<T, LPR, INTER><<<ceil_div(p.units, kWarps), kWarps * 32, 0, st>>>(p);
   } else {
-    append8_page_kernel<T, LPR, INTER>
-        <<<dim3((unsigned)tasks, p.heads, halves), kWarps * 32, 0, st>>>(p);
+    constexpr int kSmem = 2 * kKeep<T> * 2 * kPageWarps * 32 * kE * (int)sizeof(T);
+    auto kernel = append8_page_kernel<T, LPR, INTER>;
+    MSA_CUDA_RETURN(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    p.units = (uint32_t)(tasks * p.heads * halves);
+    p.by_page_parts = FastDiv((uint32_t)(p.heads * halves));
+    kernel<<<std::min<uint32_t>(p.units, 148 * kPageBlocks), kPageWarps * 32, kSmem, st>>>(p);
   }
+  return MSA_OK;
 }
 
 template <typename T>
 int launch(Params p, int halves, int dtype, bool quantised, cudaStream_t st) {
   // pages that the new tokens can touch, see find_task
   const int64_t tasks = p.cu ? p.tokens / p.page_size + 2 * (int64_t)p.batch : p.batch;
-  MSA_CHECK_ARG(tasks < (int64_t)1 << 31 && p.heads <= 65535, "msa_cache_append: too many pages or heads");
+  MSA_CHECK_ARG(tasks * p.heads * halves < (int64_t)1 << 31 && p.heads <= 65535,
+                "msa_cache_append: too many pages or heads");
   if (fast_shape(p, halves, dtype, quantised)) {
     const int lpr = p.dim <= 32 ? 4 : p.dim <= 64 ? 8 : p.dim <= 128 ? 16 : 32;
     p.head_chunks = ceil_div(p.heads, 32 / lpr * kRowsPerLane);
@@ -426,9 +554,10 @@ int launch(Params p, int halves, int dtype, bool quantised, cudaStream_t st) {
     const int64_t units = quantised ? (int64_t)p.batch * p.heads * halves : p.tokens * p.chunks;
     MSA_CHECK_ARG(units < (int64_t)1 << 31, "msa_cache_append: too many tokens * heads");
     p.units = (uint32_t)units;
-#define MSA_LAUNCH(LPR)                                                  \
-  if (p.interleaved) launch_fast<T, LPR, true>(p, halves, quantised, tasks, st); \
-  else launch_fast<T, LPR, false>(p, halves, quantised, tasks, st)
+#define MSA_LAUNCH(LPR)                                                                   \
+  status = p.interleaved ? launch_fast<T, LPR, true>(p, halves, quantised, tasks, st) \
+                         : launch_fast<T, LPR, false>(p, halves, quantised, tasks, st)
+    int status;
     switch (lpr) {
       case 4: MSA_LAUNCH(4); break;
       case 8: MSA_LAUNCH(8); break;
@@ -436,6 +565,7 @@ int launch(Params p, int halves, int dtype, bool quantised, cudaStream_t st) {
       default: MSA_LAUNCH(32); break;
     }
 #undef MSA_LAUNCH
+    if (status) return status;
   } else {
     append_any_kernel<T><<<dim3((unsigned)tasks, p.heads, halves), kWarps * 32, 0, st>>>(p);
   }
@@ -477,6 +607,7 @@ extern "C" int msa_cache_append(const void* k, const void* v, int dtype, int64_t
   p.table = rope_table, p.cu = cu_seqlens, p.block_table = block_table, p.seq_lens = seq_lens;
   p.table_rows = table_rows, p.tokens = total_tokens, p.num_pages = num_pages;
   p.batch = batch, p.heads = heads, p.dim = head_dim, p.page_size = page_size, p.max_pages = max_pages;
+  p.by_page = FastDiv((uint32_t)page_size);
   p.interleaved = interleaved != 0;
   const int halves = v ? 2 : 1;
   cudaStream_t st = as_stream(stream);

@@ -108,6 +108,21 @@ __device__ __forceinline__ double warp_max(double v) {
   return v;
 }
 
+// Division by a number that the host knows, for 0 <= n < 2^31: with s = ceil(log2 d) and
+// mul = floor(2^32 (2^s - d) / d) + 1, (mulhi(n, mul) + n) >> s is the exact quotient of every 32-bit n, and the
+// sum does not overflow below 2^31.
+struct FastDiv {
+  uint32_t mul = 1, shift = 0;
+  FastDiv() = default;
+  explicit FastDiv(uint32_t d) {
+    while (((uint64_t)1 << shift) < d) ++shift;
+    mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << shift) - d)) / d + 1);
+  }
+  __device__ __forceinline__ int operator()(int n) const {
+    return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
+  }
+};
+
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 
 }  // namespace msa

@@ -56,16 +56,10 @@ struct Params {
   float* lse;
   int64_t num_pages;
   int q_heads, groups, dim, page_size, max_pages, topk, block, split_shift, dtype;  // 2^split_shift blocks a cluster
-  uint32_t page_mul, page_shift;  // division by page_size, see page_of
+  FastDiv by_page;
   float scale_log2;
   bool uniform;  // 16 keys in a row never leave a page
 };
-
-// token / page_size for 0 <= token < 2^31: with s = ceil(log2 d) and mul = floor(2^32 (2^s - d) / d) + 1,
-// (mulhi(n, mul) + n) >> s is the exact quotient of every 32-bit n, and the sum does not overflow below 2^31.
-__device__ __forceinline__ int page_of(const Params& p, int token) {
-  return (int)((__umulhi((uint32_t)token, p.page_mul) + (uint32_t)token) >> p.page_shift);
-}
 
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
@@ -355,7 +349,7 @@ decode8_kernel(const __grid_constant__ Params p) {
       const int slot = tile / per_block, in_block = (tile - slot * per_block) * kTile + lane;
       const int64_t token = (int64_t)slots[slot] * p.block + in_block;
       if (in_block >= p.block || token > pos) return r;
-      const int logical = page_of(p, (int)token);  // token <= pos fits 32 bits
+      const int logical = p.by_page((int)token);  // token <= pos fits 32 bits
       r.row = (int)token - logical * p.page_size;
       if (logical < p.max_pages) r.page = p.block_table[(int64_t)b * p.max_pages + logical];
       return r;
@@ -749,9 +743,7 @@ extern "C" int msa_decode_attn_e4m3(const void* q, int dtype, const void* k_cach
   int splits = 1;
   while (splits < kMaxSplits && (int64_t)batch * groups * splits < 148 * 6 && splits * kWarps < tiles)
     splits *= 2, ++p.split_shift;
-  p.page_shift = 0;
-  while (((uint32_t)1 << p.page_shift) < (uint32_t)page_size) ++p.page_shift;
-  p.page_mul = (uint32_t)((((uint64_t)1 << 32) * (((uint64_t)1 << p.page_shift) - page_size)) / page_size + 1);
+  p.by_page = FastDiv((uint32_t)page_size);
   p.uniform = page_size % 16 == 0 && block_size % 16 == 0;
   const bool vec = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(k_cache) % 16 == 0 &&

@@ -21,6 +21,13 @@ __device__ __forceinline__ float scale_for(float amax) {
 
 __device__ __forceinline__ bool finite(float x) { return fabsf(x) <= 3.402823466e38f; }
 
+// Two values that lie within the scale (or are NaN) to two codes, the first in the low byte.
+__device__ __forceinline__ uint32_t encode2(float a, float b) {
+  uint16_t c;
+  asm("cvt.rn.satfinite.e4m3x2.f32 %0, %2, %1;" : "=h"(c) : "f"(a), "f"(b));
+  return c;
+}
+
 // Four values / scale to four codes, nearest even; what is not finite becomes the NaN code.
 __device__ __forceinline__ uint32_t encode4(float a, float b, float c, float d, float inv_scale) {
   const float nan = __int_as_float(0x7fc00000);

@@ -230,6 +230,22 @@ __device__ __forceinline__ float dot_of(const Lane& x, const Lane& y) {
   return t.x + t.y;
 }
 
+__device__ __forceinline__ F2 add2(F2 a, F2 b) {
+  F2 r;
+  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
+  return r;
+}
+// rotate_pair, two pairs to an instruction and with its roundings.
+__device__ __forceinline__ void rotate_exact(Lane& x, const float (&c)[kE], const float (&s)[kE]) {
+#pragma unroll
+  for (int i = 0; i < kE / 2; ++i) {
+    const F2 cc = pack2(c[2 * i], c[2 * i + 1]), ss = pack2(s[2 * i], s[2 * i + 1]),
+             minus = pack2(-s[2 * i], -s[2 * i + 1]), a = x.v[i], b = x.v[kE / 2 + i];
+    x.v[i] = add2(mul2(a, cc), mul2(b, minus));
+    x.v[kE / 2 + i] = add2(mul2(b, cc), mul2(a, ss));
+  }
+}
+
 // ------------------------------------------------------------------ shapes the lane layout does not cover
 // Unit u of a row: the pair u of the rotated elements, or one element behind them.
 struct Unit {
