@@ -23,8 +23,9 @@ import torch
 
 from . import _lib
 from ._lib import DTYPE_CODE, E4M3_CODE, call, device_of, ptr, stream_of
-from .decode import CACHE_8BIT, _check_paged, check_scale
-from .qk_norm_rope import check_table, dense_rows
+from .decode import CACHE_8BIT, _check_paged, check_scale, dense_rows
+from .qk_norm_rope import check_table
+
 
 def _check_cache(name, x, cache, scale, device):
     if cache.ndim != 4 or cache.shape[2:] != x.shape[1:]:
@@ -40,6 +41,8 @@ def _check_cache(name, x, cache, scale, device):
     elif scale is not None:
         raise ValueError(f"{name}_scale belongs to an 8-bit cache")
     # written in place: head rows must be dense, and no two elements may share memory
+    if cache.is_contiguous():
+        return
     if cache.shape[3] > 1 and cache.stride(3) != 1:
         raise ValueError(f"{name}_cache must have dense head rows")
     span = 1
@@ -106,17 +109,23 @@ def m3_cache_append(
     if rope_table is not None:
         check_table(rope_table, dim, k.device)
     _lib.require_cuda(k)
-    kd, vd = dense_rows(k), None if v is None else dense_rows(v)
-    table = None if rope_table is None else rope_table.contiguous()
-    rows, rotary = (0, 0) if table is None else table.shape
-    # held by name until the launch: a temporary's memory would be handed to the next copy
-    cu = None if cu_seqlens is None else cu_seqlens.contiguous()
-    pages, lens = block_table.contiguous(), seq_lens.contiguous()
-    v_strides = (0, 0) if v is None else (vd.stride(0), vd.stride(1))
-    v_cache_strides = (0, 0, 0) if v is None else v_cache.stride()[:3]
+    # every copy is held by name until the launch: a temporary's memory would be handed to the next one
+    k = dense_rows(k)
+    v_args = (0, 0), (0, 0, 0)
+    if v is not None:
+        v = dense_rows(v)
+        v_args = v.stride()[:2], v_cache.stride()[:3]
+    rows = rotary = 0
+    if rope_table is not None:
+        rope_table = rope_table.contiguous()
+        rows, rotary = rope_table.shape
+    if cu_seqlens is not None:
+        cu_seqlens = cu_seqlens.contiguous()
+    block_table, seq_lens = block_table.contiguous(), seq_lens.contiguous()
+    pages, page_size = k_cache.shape[:2]
     with device_of(k):
-        call("msa_cache_append", ptr(kd), ptr(vd), DTYPE_CODE[k.dtype], kd.stride(0), kd.stride(1), *v_strides,
-             ptr(table), rows, rotary, int(interleaved), ptr(cu), ptr(pages), ptr(lens), batch, total,
-             heads, dim, k_cache.shape[1], block_table.shape[1], k_cache.shape[0], ptr(k_cache), ptr(v_cache),
+        call("msa_cache_append", k.data_ptr(), ptr(v), DTYPE_CODE[k.dtype], *k.stride()[:2], *v_args[0],
+             ptr(rope_table), rows, rotary, interleaved, ptr(cu_seqlens), block_table.data_ptr(), seq_lens.data_ptr(),
+             batch, total, heads, dim, page_size, block_table.shape[1], pages, k_cache.data_ptr(), ptr(v_cache),
              E4M3_CODE if k_cache.dtype == CACHE_8BIT else DTYPE_CODE[k_cache.dtype], *k_cache.stride()[:3],
-             *v_cache_strides, ptr(k_scale), ptr(v_scale), stream_of(k))
+             *v_args[1], ptr(k_scale), ptr(v_scale), stream_of(k))

@@ -533,7 +533,8 @@ int launch_fast(Params p, int halves, bool quantised, int64_t tasks, cudaStream_
   } else {
     constexpr int kSmem = 2 * kKeep<T> * 2 * kPageWarps * 32 * kE * (int)sizeof(T);
     auto kernel = append8_page_kernel<T, LPR, INTER>;
-    MSA_CUDA_RETURN(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, kSmem));
+    static std::atomic<uint64_t> done{0};
+    MSA_CUDA_RETURN(allow_smem(kernel, kSmem, done));
     p.units = (uint32_t)(tasks * p.heads * halves);
     p.by_page_parts = FastDiv((uint32_t)(p.heads * halves));
     kernel<<<std::min<uint32_t>(p.units, 148 * kPageBlocks), kPageWarps * 32, kSmem, st>>>(p);

@@ -6,6 +6,7 @@
 #include <cuda_runtime.h>
 #include <stdint.h>
 
+#include <atomic>
 #include <cstdarg>
 #include <cstdio>
 #include <string>
@@ -122,6 +123,18 @@ struct FastDiv {
     return (int)((__umulhi((uint32_t)n, mul) + (uint32_t)n) >> shift);
   }
 };
+
+// Dynamic shared memory above 48 KB is allowed per kernel and device; `done` keeps the devices that have it.
+template <typename K>
+inline cudaError_t allow_smem(K kernel, int bytes, std::atomic<uint64_t>& done) {
+  int dev = 0;
+  if (cudaError_t e = cudaGetDevice(&dev)) return e;
+  const uint64_t bit = (uint64_t)1 << (dev & 63);
+  if (done.load(std::memory_order_acquire) & bit) return cudaSuccess;
+  if (cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, bytes)) return e;
+  done.fetch_or(bit, std::memory_order_release);
+  return cudaSuccess;
+}
 
 inline int ceil_div(int64_t a, int64_t b) { return (int)((a + b - 1) / b); }
 

@@ -685,8 +685,10 @@ template <int DP, int HR, bool SPLIT, bool VEC>
 int launch(const Params& p, int batch, cudaStream_t st) {
   const size_t smem = (size_t)kWarps * Layout<DP, HR>::kBytes + Layout<DP, HR>::kInbox;
   auto kernel = decode8_kernel<DP, HR, SPLIT, VEC>;
-  if (smem > 48 * 1024)
-    MSA_CUDA_RETURN(cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, (int)smem));
+  if (smem > 48 * 1024) {
+    static std::atomic<uint64_t> done{0};
+    MSA_CUDA_RETURN(allow_smem(kernel, (int)smem, done));
+  }
   cudaLaunchConfig_t cfg{};
   cfg.gridDim = dim3((unsigned)(batch * p.groups) << p.split_shift, (unsigned)ceil_div(p.q_heads / p.groups, 16));
   cfg.blockDim = dim3(kWarps * 32);

@@ -91,6 +91,11 @@ def m3_topk_decode(scores, seq_lens, *, block_size=128, topk_blocks=16, local_bl
 CACHE_8BIT = torch.float8_e4m3fn
 
 
+def dense_rows(x: torch.Tensor) -> torch.Tensor:
+    """``x`` itself when the rows of its last dimension are dense, else a contiguous copy."""
+    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
+
+
 def check_scale(name, scale, cache):
     """The scales of an 8-bit cache ``[P, S, G, D]``: float32 ``[P, G]``, dense."""
     if scale is None or scale.shape != (cache.shape[0], cache.shape[2]) or scale.dtype != torch.float32:
@@ -101,7 +106,6 @@ def check_scale(name, scale, cache):
         raise ValueError(f"{name} must be contiguous")
 
 
-@torch.no_grad()
 def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, block_size=128, scale=None,
                      return_lse=False, k_scale=None, v_scale=None):
     """Sparse attention of each request's new token over its selected cached blocks.
@@ -132,12 +136,13 @@ def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, blo
     if not math.isfinite(effective):
         raise ValueError("scale must be finite.")
     _check_paged(block_table, seq_lens, batch, q.device)
-    if quantised and any(x.device != q.device for x in (k_cache, v_cache, indices)):
+    if quantised and (k_cache.device != q.device or v_cache.device != q.device or indices.device != q.device):
         raise ValueError("All inputs must reside on the same device.")
     _lib.require_cuda(q)
     if quantised:
         return _sparse_decode8(q, k_cache, v_cache, block_table, seq_lens, indices, block_size, effective, return_lse,
                                k_scale, v_scale)
+    q, k_cache, v_cache = q.detach(), k_cache.detach(), v_cache.detach()
     out = torch.empty_like(q)
     lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device)
     if batch:
@@ -156,14 +161,17 @@ def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, blo
 def _sparse_decode8(q, k_cache, v_cache, block_table, seq_lens, indices, block_size, scale, return_lse, k_scale,
                     v_scale):
     batch, hq, dim = q.shape
-    out = q.new_empty(q.shape)
-    lse = q.new_empty((batch, hq), dtype=torch.float32)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device)
     if batch and dim:
-        dense = [x if x.shape[3] == 1 or x.stride(3) == 1 else x.contiguous() for x in (k_cache, v_cache)]
-        qc, table, lens, ids = q.contiguous(), block_table.contiguous(), seq_lens.contiguous(), indices.contiguous()
+        # every copy is held by name until the launch: a temporary's memory would be handed to the next one
+        q, k_cache, v_cache = q.contiguous(), dense_rows(k_cache), dense_rows(v_cache)
+        block_table, seq_lens, indices = block_table.contiguous(), seq_lens.contiguous(), indices.contiguous()
+        pages, page_size, groups, _ = k_cache.shape
         with device_of(q):
-            call("msa_decode_attn_e4m3", ptr(qc), DTYPE_CODE[q.dtype], ptr(dense[0]), ptr(dense[1]),
-                 *dense[0].stride()[:3], *dense[1].stride()[:3], ptr(k_scale), ptr(v_scale), ptr(table), ptr(lens),
-                 ptr(ids), batch, hq, k_cache.shape[2], dim, k_cache.shape[1], table.shape[1], k_cache.shape[0],
-                 ids.shape[2], block_size, scale, ptr(out), ptr(lse), stream_of(q))
+            call("msa_decode_attn_e4m3", q.data_ptr(), DTYPE_CODE[q.dtype], k_cache.data_ptr(), v_cache.data_ptr(),
+                 *k_cache.stride()[:3], *v_cache.stride()[:3], k_scale.data_ptr(), v_scale.data_ptr(),
+                 block_table.data_ptr(), seq_lens.data_ptr(), indices.data_ptr(), batch, hq, groups, dim, page_size,
+                 block_table.shape[1], pages, indices.shape[2], block_size, scale, out.data_ptr(), lse.data_ptr(),
+                 stream_of(q))
     return (out, lse) if return_lse else out

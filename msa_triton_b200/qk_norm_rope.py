@@ -24,6 +24,7 @@ import torch
 
 from . import _lib
 from ._lib import DTYPE_CODE, call, device_of, ptr, stream_of
+from .decode import dense_rows
 from .layout import sequence_lengths
 
 MAX_HEAD_DIM = 512
@@ -56,17 +57,12 @@ def check_table(rope_table, head_dim, device):
         raise ValueError("All inputs must reside on the same device.")
 
 
-def dense_rows(x: torch.Tensor) -> torch.Tensor:
-    """``x`` itself when the rows of its last dimension are dense, else a contiguous copy."""
-    return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
-
-
 def _common(q, k, q_weight, k_weight, table, positions, cu, interleaved):
     """The arguments that both launchers pass between the tensors and the strides."""
     nseq = 0 if cu is None else cu.numel() - 1
-    return (DTYPE_CODE[q.dtype], ptr(q_weight), ptr(k_weight), DTYPE_CODE[q_weight.dtype], ptr(table),
-            table.shape[0], table.shape[1], int(interleaved), ptr(positions), ptr(cu), nseq, q.shape[0], q.shape[1],
-            k.shape[1], q.shape[2], q.stride(0), q.stride(1), k.stride(0), k.stride(1))
+    return (DTYPE_CODE[q.dtype], q_weight.data_ptr(), k_weight.data_ptr(), DTYPE_CODE[q_weight.dtype],
+            table.data_ptr(), *table.shape, interleaved, ptr(positions), ptr(cu), nseq, q.shape[0], q.shape[1],
+            k.shape[1], q.shape[2], *q.stride()[:2], *k.stride()[:2])
 
 
 def _laid_out(q, k, q_weight, k_weight, table, positions, cu):
@@ -77,11 +73,11 @@ def _laid_out(q, k, q_weight, k_weight, table, positions, cu):
 def norm_rope_forward(q, k, q_weight, k_weight, table, positions, cu, eps, interleaved):
     """(q_out, k_out); shared by the autograd Function and the torch.library operator."""
     q, k, q_weight, k_weight, table, positions, cu = _laid_out(q, k, q_weight, k_weight, table, positions, cu)
-    q_out, k_out = q.new_empty(q.shape), k.new_empty(k.shape)
+    q_out, k_out = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
     with device_of(q):
-        call("msa_qk_norm_rope_fwd", ptr(q), ptr(k), *_common(q, k, q_weight, k_weight, table, positions, cu,
+        call("msa_qk_norm_rope_fwd", q.data_ptr(), k.data_ptr(), *_common(q, k, q_weight, k_weight, table, positions, cu,
                                                               interleaved),
-             float(eps), ptr(q_out), ptr(k_out), stream_of(q))
+             eps, q_out.data_ptr(), k_out.data_ptr(), stream_of(q))
     return q_out, k_out
 
 
@@ -91,13 +87,14 @@ def norm_rope_backward(q, k, q_weight, k_weight, table, positions, cu, eps, inte
         return None, None, None, None
     q, k, q_weight, k_weight, table, positions, cu = _laid_out(q, k, q_weight, k_weight, table, positions, cu)
     gq, gk = dense_rows(grad_q.to(q.dtype)), dense_rows(grad_k.to(k.dtype))
-    dq, dk, dwq, dwk = (x.new_empty(x.shape) if n else None for x, n in zip((q, k, q_weight, k_weight), need))
+    dq, dk, dwq, dwk = (torch.empty_like(x, memory_format=torch.contiguous_format) if n else None
+                        for x, n in zip((q, k, q_weight, k_weight), need))
     ws_bytes = _lib.load().msa_qk_norm_rope_bwd_workspace_size(q.shape[2]) if need[2] or need[3] else 0
     workspace = q.new_empty(ws_bytes, dtype=torch.uint8) if ws_bytes else None
     with device_of(q):
-        call("msa_qk_norm_rope_bwd", ptr(q), ptr(k), ptr(gq), ptr(gk),
-             *_common(q, k, q_weight, k_weight, table, positions, cu, interleaved), gq.stride(0), gq.stride(1),
-             gk.stride(0), gk.stride(1), float(eps), ptr(dq), ptr(dk), ptr(dwq), ptr(dwk), ptr(workspace), ws_bytes,
+        call("msa_qk_norm_rope_bwd", q.data_ptr(), k.data_ptr(), gq.data_ptr(), gk.data_ptr(),
+             *_common(q, k, q_weight, k_weight, table, positions, cu, interleaved), *gq.stride()[:2],
+             *gk.stride()[:2], eps, ptr(dq), ptr(dk), ptr(dwq), ptr(dwk), ptr(workspace), ws_bytes,
              stream_of(q))
     return dq, dk, dwq, dwk
 
@@ -155,7 +152,7 @@ def m3_qk_norm_rope(
     check_table(rope_table, dim, q.device)
     if (cu_seqlens is None) == (positions is None):
         raise ValueError("give either cu_seqlens or positions")
-    if any(x.device != q.device for x in (k, q_weight, k_weight)):
+    if k.device != q.device or q_weight.device != q.device or k_weight.device != q.device:
         raise ValueError("All inputs must reside on the same device.")
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be finite and nonnegative")
@@ -174,6 +171,7 @@ def m3_qk_norm_rope(
         from . import library
 
         return library.qk_norm_rope(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, interleaved)
-    if not (torch.is_grad_enabled() and any(x.requires_grad for x in (q, k, q_weight, k_weight))):
+    if not (torch.is_grad_enabled()
+            and (q.requires_grad or k.requires_grad or q_weight.requires_grad or k_weight.requires_grad)):
         return norm_rope_forward(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, interleaved)
     return _QKNormRope.apply(q, k, q_weight, k_weight, rope_table, positions, cu_seqlens, eps, bool(interleaved))
