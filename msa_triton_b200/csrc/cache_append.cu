@@ -16,6 +16,7 @@
 //
 // A page that receives tokens belongs to one request (shared prefix pages are full ones).
 #include <algorithm>
+#include <type_traits>
 
 #include "e4m3.cuh"
 #include "rope_common.cuh"
@@ -27,11 +28,7 @@ using namespace rope;
 
 constexpr int kWarps = 8;
 constexpr int kRowsPerLane = 4;
-constexpr int kPageWarps = 8;
-// Blocks to an SM: 3 with a few spilled registers 75 us at 32768 tokens of 8 heads of 128, 2 without 87 us.
-constexpr int kPageBlocks = 3;
-template <typename T>
-constexpr int kKeep = sizeof(T) == 4 ? 4 : 8;  // rows of a page that a lane holds between the two passes
+constexpr int kPageBlocks = 4;  // of the page kernel, to an SM (3: 67 us, 4: 62 us at 32768 tokens of 8 heads of 128)
 constexpr int kMaxDimFast = 256;
 
 struct Half {  // k or v
@@ -263,12 +260,6 @@ __global__ void __launch_bounds__(kWarps * 32) append8_token_kernel(const __grid
   if (lane == 0 && now != old) *scale = now;
 }
 
-template <int BYTES>
-__device__ __forceinline__ void copy_run(uint32_t to, const void* from) {
-  asm volatile("cp.async.ca.shared.global [%0], [%1], %2;" ::"r"(to), "l"(from), "n"(BYTES) : "memory");
-}
-
-template <int WARPS>
 __device__ __forceinline__ float block_amax(float v, float* red) {
 #pragma unroll
   for (int o = 16; o > 0; o >>= 1) v = fmaxf(v, __shfl_xor_sync(0xffffffffu, v, o));
@@ -276,170 +267,140 @@ __device__ __forceinline__ float block_amax(float v, float* red) {
   __syncthreads();
   v = red[0];
 #pragma unroll
-  for (int w = 1; w < WARPS; ++w) v = fmaxf(v, red[w]);
+  for (int w = 1; w < kWarps; ++w) v = fmaxf(v, red[w]);
   return v;
 }
 
-// Chunks: an item of work is a (request, page, head) of k or v, the heads of a page one after the other (their
-// rows lie side by side in memory). Blocks stay and walk over the items. Every thread copies the runs of its
-// rows of the next item into places of its own in shared memory (cp.async: nothing to wait for but its own
-// copies), while it rotates the current ones into registers, takes the page's maximum and writes the codes. Rows past kKeep a
-// lane (pages longer than 128 rows of 128) are read twice from memory instead. The maximum takes whatever is
-// there: NaN drops out of fmaxf by itself, and only a page that holds an infinity is looked through again
-// for its finite values.
-// (Giving a block several heads of a page in a row keeps the angles in L1 but scatters the reads: 101 us
-// with four heads, 123 us with eight, at the sizes below.)
-template <typename T, int LPR, bool INTER>
-__global__ void __launch_bounds__(kPageWarps * 32, kPageBlocks) append8_page_kernel(const __grid_constant__ Params p) {
-  constexpr int kThreads = kPageWarps * 32, kRows = kThreads / LPR, kHeld = kKeep<T>, kRun = kE * (int)sizeof(T);
-  extern __shared__ __align__(16) uint8_t smem[];  // [2][kHeld][2][kThreads] runs
-  __shared__ float red[2][kPageWarps];
+// Chunks: a block takes HC heads (4, or 1 of a tensor with fewer) of a (request, page), of k or v. It reads the rows
+// twice, once for the heads' maxima and once for the codes: the second time they come from L2 (a wave of blocks
+// holds some 50 MB, half the L2). That keeps whole kilobytes of a token's heads together and one set of angles for
+// them, and holds nothing on the way. The maximum takes whatever is there: NaN drops out of fmaxf by itself, and
+// only a page that holds an infinity is looked through again for its finite values.
+template <typename T, int LPR, bool INTER, int HC>
+__global__ void __launch_bounds__(kWarps * 32, kPageBlocks) append8_page_kernel(const __grid_constant__ Params p) {
+  constexpr int kRows = kWarps * 32 / LPR;  // tokens of a step
+  __shared__ float red[kWarps][HC], inverse[HC], ratio[HC];
+  __shared__ bool infinite[HC];
+  const int task = p.by_page_parts((int)blockIdx.x), part = (int)blockIdx.x - task * (int)(p.chunks * p.head_chunks);
+  Task t;
+  if (!find_task(p, task, t)) return;  // the same for the whole block
+  const int64_t at = physical_page(p, t.b, t.logical);
+  if (at < 0) return;
+  const bool is_v = part >= (int)p.head_chunks;
+  const Half& s = p.half[is_v];
+  const int h0 = (part - is_v * (int)p.head_chunks) * HC, heads = min(HC, p.heads - h0);
   const int tid = threadIdx.x, l = tid % LPR, r0 = tid / LPR;
-  const uint32_t place = (uint32_t)__cvta_generic_to_shared(smem) + tid * kRun;
+  const LaneMap m = lane_map<INTER>(l, p.dim, s.rotary);
+  const bool turned = m.rotated && s.rotary > 0;
+  // rows from here on have no angle
+  const int inside = s.rotary > 0 ? (int)min(max(p.table_rows - t.pos, (int64_t)0), (int64_t)t.n) : t.n;
+  float old = 0.f;
+  if (tid < heads) old = s.scale[at * p.heads + h0 + tid];
 
-  struct Item {
-    Task t;
-    int h;
-    bool is_v, some;
-  };
-  auto item_of = [&](uint32_t i) {
-    Item it;
-    it.some = i < p.units;
-    if (!it.some) return it;
-    const int task = p.by_page_parts((int)i), part = (int)i - task * (p.heads * (int)p.chunks);
-    it.is_v = part >= p.heads;
-    it.h = part - it.is_v * p.heads;
-    it.some = find_task(p, task, it.t);
-    return it;
-  };
-  auto issue = [&](const Item& it, int buffer) {
-    if (it.some) {
-      const Half& s = p.half[it.is_v];
-      const LaneMap m = lane_map<INTER>(l, p.dim, s.rotary);
-      const T* x = static_cast<const T*>(s.x) + (it.t.token + r0) * s.x_ts + it.h * s.x_hs + m.a;
-      const int n = m.active ? min(it.t.n, kHeld * kRows) : 0, d = m.b - m.a;
-      uint32_t to = place + buffer * (kHeld * 2 * kThreads * kRun);
+  // Calls f(head, values, code row) for the lane's rotated values of every row.
+  uint8_t* const page = static_cast<uint8_t*>(s.cache) + at * s.c_ps + h0 * s.c_hs;
+  auto visit = [&](auto again, auto f) {
+    const T* x = static_cast<const T*>(s.x) + (t.token + r0) * s.x_ts + h0 * s.x_hs + m.a;
+    const int64_t to_b = m.b - m.a, step = kRows * s.x_ts, out_step = kRows * s.c_ts;
+    const float* angle = turned ? p.table + (int64_t)(t.pos + r0) * s.rotary + kE * l : nullptr;
+    uint8_t* out = page + (int64_t)(t.row_first + r0) * s.c_ts;
+    for (int r = r0; r < t.n; r += kRows) {
+      Raw<T> raw[HC][2];
+      const T* row = x;
 #pragma unroll
-      for (int i = 0; i < kHeld; ++i) {
-        if (r0 + i * kRows < n) {
-          copy_run<kRun>(to, x);
-          copy_run<kRun>(to + kThreads * kRun, x + d);
+      for (int i = 0; i < HC; ++i) {
+        raw[i][0].u = raw[i][1].u = {};
+        if (i < heads && m.active) {
+          raw[i][0] = again ? load_run_again(row) : load_run(row);
+          raw[i][1] = again ? load_run_again(row + to_b) : load_run(row + to_b);
         }
-        x += kRows * s.x_ts;
-        to += 2 * kThreads * kRun;
+        row += s.x_hs;
       }
+      Angle2 angles;
+      if (turned && r < inside) angles.load(angle, angle + s.rotary / 2);
+      uint8_t* to = out;
+#pragma unroll
+      for (int i = 0; i < HC; ++i) {
+        float v[2 * kE];
+        unpack_lane<INTER>(raw[i], v);
+        Lane y = lane_of(v);
+        if (r >= inside) {
+#pragma unroll
+          for (int e = 0; e < kE; ++e) y.v[e] = twice(nan_f32());
+        } else if (turned) {
+          rotate_exact(y, angles);
+        }
+        if (i < heads && m.active) f(i, y, to);
+        to += s.c_hs;
+      }
+      x += step;
+      out += out_step;
+      angle += kRows * s.rotary;
     }
-    asm volatile("cp.async.commit_group;" ::: "memory");
   };
-
-  uint32_t index = blockIdx.x;
-  Item now = item_of(index);
-  issue(now, 0);
-  for (int turn = 0; index < p.units; turn ^= 1) {
-    index += gridDim.x;
-    const Item next = item_of(index);
-    issue(next, turn ^ 1);
-    asm volatile("cp.async.wait_group 1;" ::: "memory");
-    const Item it = now;
-    now = next;
-    if (!it.some) continue;  // the same for the whole block
-    const int64_t at = physical_page(p, it.t.b, it.t.logical);
-    if (at < 0) continue;
-    const Half& s = p.half[it.is_v];
-    const LaneMap m = lane_map<INTER>(l, p.dim, s.rotary);
-    float* scale = s.scale + at * p.heads + it.h;
-    const float old = *scale;
-    const int n = it.t.n, held = m.active ? min(n, kHeld * kRows) : 0;
-    const bool turned = m.rotated && s.rotary > 0;
-    // rows from here on have no angle
-    const int inside = s.rotary > 0 ? (int)min(max(p.table_rows - it.t.pos, (int64_t)0), (int64_t)n) : n;
-    const float* angles = turned ? p.table + (int64_t)(it.t.pos + r0) * s.rotary + kE * l : nullptr;
-    const uint8_t* mine = smem + tid * kRun + turn * (kHeld * 2 * kThreads * kRun);
-    auto turn_row = [&](Lane y, int r, const float* angle) {
-      if (r >= inside) {
+  // The heads' maxima, with or without infinite values, in red[0].
+  auto maxima = [&](auto finite) {
+    float amax[HC];
 #pragma unroll
-        for (int i = 0; i < kE; ++i) y.v[i] = twice(nan_f32());
-      } else if (turned) {
-        const float4 c = __ldg(reinterpret_cast<const float4*>(angle));
-        const float4 sn = __ldg(reinterpret_cast<const float4*>(angle + s.rotary / 2));
-        const float cc[kE] = {c.x, c.y, c.z, c.w}, ss[kE] = {sn.x, sn.y, sn.z, sn.w};
-        rotate_exact(y, cc, ss);
+    for (int i = 0; i < HC; ++i) amax[i] = 0.f;
+    visit(std::true_type(), [&](int i, const Lane& y, uint8_t*) {
+#pragma unroll
+      for (int e = 0; e < kE; ++e) {
+        const float2 f = unpack2(y.v[e]);
+        amax[i] = fmaxf(amax[i], finite && !e4m3::finite(f.x) ? 0.f : fabsf(f.x));
+        amax[i] = fmaxf(amax[i], finite && !e4m3::finite(f.y) ? 0.f : fabsf(f.y));
       }
-      return y;
-    };
-    auto held_row = [&](int i) {
-      const Raw<T>* from = reinterpret_cast<const Raw<T>*>(mine + i * (2 * kThreads * kRun));
-      const Raw<T> raw[2] = {from[0], from[kThreads]};
-      float f[2 * kE];
-      unpack_lane<INTER>(raw, f);
-      return turn_row(lane_of(f), r0 + i * kRows, angles + i * (kRows * s.rotary));
-    };
-    auto reread = [&](int r) {
-      const T* x = static_cast<const T*>(s.x) + (it.t.token + r) * s.x_ts + it.h * s.x_hs;
-      const Raw<T> raw[2] = {load_run(x + m.a), load_run(x + m.b)};
-      float f[2 * kE];
-      unpack_lane<INTER>(raw, f);
-      return turn_row(lane_of(f), r, p.table + (int64_t)(it.t.pos + r) * s.rotary + kE * l);
-    };
-    // the largest magnitude, with or without the infinite ones
-    auto largest = [&](const Lane& v, float acc, bool finite) {
+    });
 #pragma unroll
-      for (int i = 0; i < kE; ++i) {
-        const float2 f = unpack2(v.v[i]);
-        acc = fmaxf(acc, finite && !e4m3::finite(f.x) ? 0.f : fabsf(f.x));
-        acc = fmaxf(acc, finite && !e4m3::finite(f.y) ? 0.f : fabsf(f.y));
-      }
-      return acc;
-    };
-    Lane y[kHeld];
+    for (int i = 0; i < HC; ++i) {
 #pragma unroll
-    for (int i = 0; i < kHeld; ++i)
-      if (r0 + i * kRows < held) y[i] = held_row(i);
-      else y[i] = Lane{};
-    auto page_amax = [&](bool finite, float* red_at) {
-      float amax = 0.f;
-#pragma unroll
-      for (int i = 0; i < kHeld; ++i) amax = largest(y[i], amax, finite);
-      if (m.active)
-        for (int r = r0 + kHeld * kRows; r < n; r += kRows) amax = largest(reread(r), amax, finite);
-      return block_amax<kPageWarps>(amax, red_at);
-    };
-    float amax = page_amax(false, red[turn]);  // two places: the next item's are written before all have read these
-    const bool infinite = amax == INFINITY;
-    if (infinite) {
-      __syncthreads();
-      amax = page_amax(true, red[turn]);
+      for (int o = 16; o > 0; o >>= 1) amax[i] = fmaxf(amax[i], __shfl_xor_sync(0xffffffffu, amax[i], o));
+      if ((tid & 31) == 0) red[tid >> 5][i] = amax[i];
     }
-    const float now_scale = grown_scale(amax, it.t.row_first, old), inv = 1.f / now_scale;
-    uint8_t* page = static_cast<uint8_t*>(s.cache) + at * s.c_ps + it.h * s.c_hs;
-    uint8_t* out = page + (it.t.row_first + r0) * s.c_ts;
-    auto put = [&](const Lane& v, uint8_t* to) {
-      float f[2 * kE], a[kE], b[kE];
-      if (infinite) {
-        floats_of(v, f);
-        store_codes<INTER>(to, m, f, inv);
-        return;
-      }
-      Lane z;
+    __syncthreads();
+    if (tid < HC) {
+      float top = red[0][tid];
 #pragma unroll
-      for (int i = 0; i < kE; ++i) z.v[i] = mul2(v.v[i], twice(inv));
-      floats_of(z, f);
-      from_pairs<INTER>(f, a, b);
-      *reinterpret_cast<uint32_t*>(to + m.a) = e4m3::encode2(a[0], a[1]) | e4m3::encode2(a[2], a[3]) << 16;
-      *reinterpret_cast<uint32_t*>(to + m.b) = e4m3::encode2(b[0], b[1]) | e4m3::encode2(b[2], b[3]) << 16;
-    };
-#pragma unroll
-    for (int i = 0; i < kHeld; ++i) {
-      if (r0 + i * kRows < held) put(y[i], out);
-      out += kRows * s.c_ts;
+      for (int w = 1; w < kWarps; ++w) top = fmaxf(top, red[w][tid]);
+      red[0][tid] = top;
     }
-    if (m.active)
-      for (int64_t r = r0 + kHeld * kRows; r < n; r += kRows, out += kRows * s.c_ts) put(reread(r), out);
-    if (it.t.row_first > 0 && now_scale > old)
-      move_rows(page, s.c_ts, (int)it.t.row_first, p.dim, old / now_scale, tid, kThreads);
-    if (tid == 0 && now_scale != old) *scale = now_scale;
+    __syncthreads();
+  };
+  maxima(std::false_type());
+  if (tid < HC) infinite[tid] = red[0][tid] == INFINITY;
+  __syncthreads();
+  bool any = false;
+#pragma unroll
+  for (int i = 0; i < HC; ++i) any = any || infinite[i];
+  if (any) maxima(std::true_type());
+  if (tid < heads) {
+    const float now = grown_scale(red[0][tid], t.row_first, old);
+    inverse[tid] = 1.f / now;
+    ratio[tid] = t.row_first > 0 && now > old ? old / now : 1.f;
+    if (now != old) s.scale[at * p.heads + h0 + tid] = now;
   }
-  asm volatile("cp.async.wait_group 0;" ::: "memory");
+  __syncthreads();
+  float inv[HC];
+#pragma unroll
+  for (int i = 0; i < HC; ++i) inv[i] = i < heads ? inverse[i] : 0.f;
+  visit(std::false_type(), [&](int i, const Lane& y, uint8_t* to) {
+    float f[2 * kE], a[kE], b[kE];
+    if (any) {
+      floats_of(y, f);
+      store_codes<INTER>(to, m, f, inv[i]);
+      return;
+    }
+    Lane z;
+#pragma unroll
+    for (int e = 0; e < kE; ++e) z.v[e] = mul2(y.v[e], twice(inv[i]));
+    floats_of(z, f);
+    from_pairs<INTER>(f, a, b);
+    *reinterpret_cast<uint32_t*>(to + m.a) = e4m3::encode2(a[0], a[1]) | e4m3::encode2(a[2], a[3]) << 16;
+    *reinterpret_cast<uint32_t*>(to + m.b) = e4m3::encode2(b[0], b[1]) | e4m3::encode2(b[2], b[3]) << 16;
+  });
+  for (int i = 0; i < heads; ++i)
+    if (ratio[i] != 1.f)
+      move_rows(page + i * s.c_hs, s.c_ts, t.row_first, p.dim, ratio[i], tid, kWarps * 32);
 }
 
 // ------------------------------------------------------------------ any shape
@@ -491,7 +452,7 @@ __global__ void __launch_bounds__(kWarps * 32) append_any_kernel(const __grid_co
     value(i, row, e, a, b);
     amax = fmaxf(amax, fmaxf(e4m3::finite(a) ? fabsf(a) : 0.f, e4m3::finite(b) ? fabsf(b) : 0.f));
   }
-  const float now = grown_scale(block_amax<kWarps>(amax, red), t.row_first, old), inv = 1.f / now;
+  const float now = grown_scale(block_amax(amax, red), t.row_first, old), inv = 1.f / now;
   uint8_t* page = static_cast<uint8_t*>(s.cache) + at * s.c_ps + h * s.c_hs;
   for (int64_t i = threadIdx.x; i < n; i += kWarps * 32) {
     value(i, row, e, a, b);
@@ -525,21 +486,21 @@ bool fast_shape(const Params& p, int halves, int dtype, bool quantised) {
 }
 
 template <typename T, int LPR, bool INTER>
-int launch_fast(Params p, int halves, bool quantised, int64_t tasks, cudaStream_t st) {
+void launch_fast(Params p, int halves, bool quantised, int64_t tasks, cudaStream_t st) {
   if (!quantised) {
     append_kernel<T, LPR, INTER><<<ceil_div(p.units, kWarps), kWarps * 32, 0, st>>>(p);
   } else if (!p.cu) {
     append8_token_kernel<T, LPR, INTER><<<ceil_div(p.units, kWarps), kWarps * 32, 0, st>>>(p);
   } else {
-    constexpr int kSmem = 2 * kKeep<T> * 2 * kPageWarps * 32 * kE * (int)sizeof(T);
-    auto kernel = append8_page_kernel<T, LPR, INTER>;
-    static std::atomic<uint64_t> done{0};
-    MSA_CUDA_RETURN(allow_smem(kernel, kSmem, done));
-    p.units = (uint32_t)(tasks * p.heads * halves);
-    p.by_page_parts = FastDiv((uint32_t)(p.heads * halves));
-    kernel<<<std::min<uint32_t>(p.units, 148 * kPageBlocks), kPageWarps * 32, kSmem, st>>>(p);
+    const int together = p.heads >= 4 ? 4 : 1;
+    p.chunks = halves;
+    p.head_chunks = ceil_div(p.heads, together);
+    const uint32_t parts = p.chunks * p.head_chunks;
+    p.by_page_parts = FastDiv(parts);
+    const unsigned blocks = (unsigned)(tasks * parts);
+    if (together == 4) append8_page_kernel<T, LPR, INTER, 4><<<blocks, kWarps * 32, 0, st>>>(p);
+    else append8_page_kernel<T, LPR, INTER, 1><<<blocks, kWarps * 32, 0, st>>>(p);
   }
-  return MSA_OK;
 }
 
 template <typename T>
@@ -556,9 +517,8 @@ int launch(Params p, int halves, int dtype, bool quantised, cudaStream_t st) {
     MSA_CHECK_ARG(units < (int64_t)1 << 31, "msa_cache_append: too many tokens * heads");
     p.units = (uint32_t)units;
 #define MSA_LAUNCH(LPR)                                                                   \
-  status = p.interleaved ? launch_fast<T, LPR, true>(p, halves, quantised, tasks, st) \
-                         : launch_fast<T, LPR, false>(p, halves, quantised, tasks, st)
-    int status;
+  if (p.interleaved) launch_fast<T, LPR, true>(p, halves, quantised, tasks, st);          \
+  else launch_fast<T, LPR, false>(p, halves, quantised, tasks, st)
     switch (lpr) {
       case 4: MSA_LAUNCH(4); break;
       case 8: MSA_LAUNCH(8); break;
@@ -566,7 +526,6 @@ int launch(Params p, int halves, int dtype, bool quantised, cudaStream_t st) {
       default: MSA_LAUNCH(32); break;
     }
 #undef MSA_LAUNCH
-    if (status) return status;
   } else {
     append_any_kernel<T><<<dim3((unsigned)tasks, p.heads, halves), kWarps * 32, 0, st>>>(p);
   }

@@ -55,7 +55,10 @@ struct Params {
   void* out;
   float* lse;
   int64_t num_pages;
-  int q_heads, groups, dim, page_size, max_pages, topk, block, split_shift, dtype;  // 2^split_shift blocks a cluster
+  int q_heads, groups, dim, page_size, max_pages, topk, block, dtype;
+  // Clusters of 2^split_shift blocks. The first `shared` items ((request, group) pairs) take a cluster each, those
+  // after them a block each.
+  int split_shift, shared;
   FastDiv by_page;
   float scale_log2;
   bool uniform;  // 16 keys in a row never leave a page
@@ -263,8 +266,10 @@ decode8_kernel(const __grid_constant__ Params p) {
   constexpr int kKT = kTile / 16;                 // 16-key tiles of S
   extern __shared__ __align__(128) uint8_t smem[];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, n = lane >> 2, j = lane & 3;
-  const int splits = 1 << p.split_shift;
-  const int split = blockIdx.x & (splits - 1), bg = blockIdx.x >> p.split_shift;
+  const int shared_blocks = p.shared << p.split_shift, behind = (int)blockIdx.x - shared_blocks;
+  const int split_shift = behind >= 0 ? 0 : p.split_shift, splits = 1 << split_shift;  // the same for a whole cluster
+  const int split = behind >= 0 ? 0 : blockIdx.x & (splits - 1);
+  const int bg = behind >= 0 ? p.shared + behind : blockIdx.x >> split_shift;
   const int b = bg / p.groups, g = bg - b * p.groups;
   const int h_all = p.q_heads / p.groups, h0 = blockIdx.y * 16, h = min(16, h_all - h0);
   if (splits > 1) cluster_arrive();  // waited for before the first store to another block
@@ -622,7 +627,7 @@ decode8_kernel(const __grid_constant__ Params p) {
   // that finishes them (element at: block at % splits)
   const uint32_t inbox = (uint32_t)__cvta_generic_to_shared(smem) + kWarps * L::kBytes;
   const uint32_t inbox_stats = inbox + kRows * DP * 4;
-  const int elements = h * (DP / 4), share = elements >> p.split_shift;  // DP / 4 is a multiple of kMaxSplits
+  const int elements = h * (DP / 4), share = elements >> split_shift;  // DP / 4 is a multiple of kMaxSplits
   if (splits > 1) cluster_wait();  // every block of the cluster has started: its memory may be written
   for (int at = threadIdx.x; at < elements; at += kWarps * 32) {
     const int row = at / (DP / 4), i = at % (DP / 4);
@@ -645,7 +650,7 @@ decode8_kernel(const __grid_constant__ Params p) {
     if (splits == 1) {
       finish(row, i, m, mv, sum, acc);
     } else {
-      store_cluster4(cluster_address(inbox, at & (splits - 1)) + 16 * (split * share + (at >> p.split_shift)), acc);
+      store_cluster4(cluster_address(inbox, at & (splits - 1)) + 16 * (split * share + (at >> split_shift)), acc);
       if (i < splits)
         store_cluster4(cluster_address(inbox_stats, i) + 16 * (split * kRows + row), make_float4(m, mv, sum, 0.f));
     }
@@ -658,7 +663,7 @@ decode8_kernel(const __grid_constant__ Params p) {
   const float4* shares = reinterpret_cast<const float4*>(smem + kWarps * L::kBytes);
   const float4* stats = shares + kRows * DP / 4;
   for (int k = threadIdx.x; k < share; k += kWarps * 32) {
-    const int at = (k << p.split_shift) + split, row = at / (DP / 4), i = at % (DP / 4);
+    const int at = (k << split_shift) + split, row = at / (DP / 4), i = at % (DP / 4);
     float4 part[kMaxSplits], s[kMaxSplits];
     float m = -INFINITY, mv = -INFINITY, sum = 0.f;
 #pragma unroll
@@ -681,16 +686,45 @@ decode8_kernel(const __grid_constant__ Params p) {
   }
 }
 
+// What a block spends outside its tiles, in tiles of a warp (start, first loads, merge: some 14,000 cycles under
+// load, against 3,200 for a tile).
+constexpr double kOverhead = 4.5;
+
 template <int DP, int HR, bool SPLIT, bool VEC>
-int launch(const Params& p, int batch, cudaStream_t st) {
+int launch(Params p, int batch, cudaStream_t st) {
   const size_t smem = (size_t)kWarps * Layout<DP, HR>::kBytes + Layout<DP, HR>::kInbox;
   auto kernel = decode8_kernel<DP, HR, SPLIT, VEC>;
   if (smem > 48 * 1024) {
     static std::atomic<uint64_t> done{0};
     MSA_CUDA_RETURN(allow_smem(kernel, (int)smem, done));
   }
+  static std::atomic<int> resident{0};  // blocks to an SM
+  int per_sm = resident.load(std::memory_order_relaxed);
+  if (per_sm == 0) {
+    MSA_CUDA_RETURN(cudaOccupancyMaxActiveBlocksPerMultiprocessor(&per_sm, kernel, kWarps * 32, smem));
+    per_sm = std::max(per_sm, 1);
+    resident.store(per_sm, std::memory_order_relaxed);
+  }
+  // Whole waves of items go a block each, which costs the least in merging; what is over and above them is
+  // split over clusters of the size that finishes first, and goes first, so that the chip is full to the end
+  // (64 requests of 8 groups and 16 blocks: 65.5 us, 67.4 with two blocks to every item; 24 requests of 2
+  // groups, a full wave or less: 11.5 against 16).
+  const int64_t head_tiles = ceil_div(p.q_heads / p.groups, 16), items = (int64_t)batch * p.groups;
+  const int64_t slots = std::max<int64_t>(148 * per_sm / head_tiles, 1);
+  const int64_t tiles = (int64_t)p.topk * ((p.block + kTile - 1) / kTile);
+  const int64_t alone = items / slots * slots;
+  int64_t shared = 0;
+  double best = 0;
+  for (int shift = 0; (1 << shift) <= kMaxSplits; ++shift) {
+    if (shift && ((int64_t)kWarps << (shift - 1)) >= tiles) break;  // no more warps than tiles
+    const int64_t rest = items - (alone >> shift << shift);           // whole clusters of lone blocks behind them
+    const double waves = (double)(((rest << shift) + slots - 1) / slots);
+    const double cost = waves * ((double)tiles / (kWarps << shift) + kOverhead);
+    if (shift == 0 || cost < best) best = cost, p.split_shift = shift, shared = shift ? rest : 0;
+  }
+  p.shared = (int)shared;
   cudaLaunchConfig_t cfg{};
-  cfg.gridDim = dim3((unsigned)(batch * p.groups) << p.split_shift, (unsigned)ceil_div(p.q_heads / p.groups, 16));
+  cfg.gridDim = dim3((unsigned)((shared << p.split_shift) + items - shared), (unsigned)head_tiles);
   cfg.blockDim = dim3(kWarps * 32);
   cfg.dynamicSmemBytes = smem;
   cfg.stream = st;
@@ -740,11 +774,6 @@ extern "C" int msa_decode_attn_e4m3(const void* q, int dtype, const void* k_cach
   p.num_pages = num_pages, p.q_heads = q_heads, p.groups = groups, p.dim = head_dim, p.page_size = page_size;
   p.max_pages = max_pages, p.topk = topk_blocks, p.block = block_size;
   p.scale_log2 = (float)(scale * 1.4426950408889634);
-  // Blocks for a (request, group): until the chip is full, and no more warps than tiles.
-  const int64_t tiles = (int64_t)topk_blocks * ((block_size + kTile - 1) / kTile);
-  int splits = 1;
-  while (splits < kMaxSplits && (int64_t)batch * groups * splits < 148 * 6 && splits * kWarps < tiles)
-    splits *= 2, ++p.split_shift;
   p.by_page = FastDiv((uint32_t)page_size);
   p.uniform = page_size % 16 == 0 && block_size % 16 == 0;
   const bool vec = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&

@@ -51,6 +51,14 @@ __device__ __forceinline__ Raw<T> load_run(const T* p) {
   return r;
 }
 
+// The same for rows that are read again soon.
+template <typename T>
+__device__ __forceinline__ Raw<T> load_run_again(const T* p) {
+  Raw<T> r;
+  r.u = __ldg(reinterpret_cast<const decltype(r.u)*>(p));
+  return r;
+}
+
 __device__ __forceinline__ void unpack_word(uint32_t w, __half, float& a, float& b) {
   const float2 f = __half22float2(*reinterpret_cast<const __half2*>(&w));
   a = f.x, b = f.y;
@@ -235,14 +243,23 @@ __device__ __forceinline__ F2 add2(F2 a, F2 b) {
   asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
   return r;
 }
+// A lane's angles, ready for rotate_exact.
+struct Angle2 {
+  F2 c[kE / 2], s[kE / 2], minus[kE / 2];
+  __device__ __forceinline__ void load(const float* cos4, const float* sin4) {
+    const float4 x = __ldg(reinterpret_cast<const float4*>(cos4)), y = __ldg(reinterpret_cast<const float4*>(sin4));
+    c[0] = pack2(x.x, x.y), c[1] = pack2(x.z, x.w);
+    s[0] = pack2(y.x, y.y), s[1] = pack2(y.z, y.w);
+    minus[0] = pack2(-y.x, -y.y), minus[1] = pack2(-y.z, -y.w);
+  }
+};
 // rotate_pair, two pairs to an instruction and with its roundings.
-__device__ __forceinline__ void rotate_exact(Lane& x, const float (&c)[kE], const float (&s)[kE]) {
+__device__ __forceinline__ void rotate_exact(Lane& x, const Angle2& t) {
 #pragma unroll
   for (int i = 0; i < kE / 2; ++i) {
-    const F2 cc = pack2(c[2 * i], c[2 * i + 1]), ss = pack2(s[2 * i], s[2 * i + 1]),
-             minus = pack2(-s[2 * i], -s[2 * i + 1]), a = x.v[i], b = x.v[kE / 2 + i];
-    x.v[i] = add2(mul2(a, cc), mul2(b, minus));
-    x.v[kE / 2 + i] = add2(mul2(b, cc), mul2(a, ss));
+    const F2 a = x.v[i], b = x.v[kE / 2 + i];
+    x.v[i] = add2(mul2(a, t.c[i]), mul2(b, t.minus[i]));
+    x.v[kE / 2 + i] = add2(mul2(b, t.c[i]), mul2(a, t.s[i]));
   }
 }
 
