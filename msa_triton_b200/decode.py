@@ -57,8 +57,9 @@ def m3_index_score_decode(index_q, index_k_cache, block_table, seq_lens, max_seq
     blocks = (max_seqlen + block_size - 1) // block_size
     scores = torch.empty((batch, groups, blocks), dtype=torch.float32, device=index_q.device)
     iq, ik = index_q.contiguous(), index_k_cache.contiguous()
+    block_table, seq_lens = block_table.contiguous(), seq_lens.contiguous()
     with torch.cuda.device(iq.device):
-        call("msa_decode_index_score", ptr(iq), ptr(ik), DTYPE_CODE[iq.dtype], ptr(block_table.contiguous()),
+        call("msa_decode_index_score", ptr(iq), ptr(ik), DTYPE_CODE[iq.dtype], ptr(block_table),
              ptr(seq_lens), batch, groups, dim, ik.shape[1], block_table.shape[1], blocks, block_size, float(scale),
              ptr(scores), stream_of(iq))
     return scores
@@ -142,18 +143,19 @@ def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, blo
     if quantised:
         return _sparse_decode8(q, k_cache, v_cache, block_table, seq_lens, indices, block_size, effective, return_lse,
                                k_scale, v_scale)
-    q, k_cache, v_cache = q.detach(), k_cache.detach(), v_cache.detach()
-    out = torch.empty_like(q)
+    out = torch.empty_like(q, memory_format=torch.contiguous_format)
     lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device)
     if batch:
         lib = _lib.load()
         topk = indices.shape[2]
         ws_bytes = lib.msa_decode_attn_workspace_size(batch, hq, dim, topk)
         ws = torch.empty(ws_bytes, dtype=torch.uint8, device=q.device)
+        # every copy is held by name until the launch: a temporary's memory would be handed to the next one
         qc, kc, vc = q.contiguous(), k_cache.contiguous(), v_cache.contiguous()
-        with torch.cuda.device(q.device):
-            call("msa_decode_attn", ptr(qc), ptr(kc), ptr(vc), DTYPE_CODE[q.dtype], ptr(block_table.contiguous()),
-                 ptr(seq_lens), ptr(indices.contiguous()), batch, hq, groups, dim, kc.shape[1], block_table.shape[1],
+        block_table, seq_lens, indices = block_table.contiguous(), seq_lens.contiguous(), indices.contiguous()
+        with device_of(q):
+            call("msa_decode_attn", ptr(qc), ptr(kc), ptr(vc), DTYPE_CODE[q.dtype], ptr(block_table),
+                 ptr(seq_lens), ptr(indices), batch, hq, groups, dim, kc.shape[1], block_table.shape[1],
                  topk, block_size, effective, ptr(out), ptr(lse), ptr(ws), ws_bytes, stream_of(q))
     return (out, lse) if return_lse else out
 
