@@ -93,6 +93,10 @@ def m3_cache_append(
         _check_cache("v", v, v_cache, v_scale, k.device)
         if v_cache.shape[:2] != k_cache.shape[:2] or v_cache.dtype != k_cache.dtype:
             raise ValueError("k_cache and v_cache must share their pages and dtype")
+        if (v_cache.data_ptr() == k_cache.data_ptr() and k_cache.numel()) or (v_scale is not None
+                                                                             and v_scale.data_ptr() == k_scale.data_ptr()
+                                                                             and k_scale.numel()):
+            raise ValueError("k and v need caches and scales of their own")
     elif v_scale is not None:
         raise ValueError("v_scale belongs to an 8-bit cache")
     if seq_lens.ndim != 1:

@@ -65,6 +65,9 @@ def test_rope_table():
             m3_rope_table(**bad)
 
 
+ONE_CACHE, ONE_SCALE = torch.zeros(4, 8, 2, 16), torch.ones(4, 2)
+
+
 def append_args(**kw):
     a = dict(k=torch.ones(2, 2, 16), v=torch.ones(2, 2, 16), k_cache=torch.zeros(4, 8, 2, 16),
              v_cache=torch.zeros(4, 8, 2, 16), block_table=torch.zeros(2, 2, dtype=torch.int32),
@@ -98,6 +101,8 @@ def eight(**kw):
     (ValueError, "k_scale must be", eight(k_scale=torch.ones(4, 2).double())),
     (ValueError, "k_scale must be contiguous", eight(k_scale=torch.ones(2, 4).t())),
     (ValueError, "v_scale belongs", dict(v=None, v_cache=None, v_scale=torch.ones(4, 2))),
+    (ValueError, "of their own", dict(k_cache=ONE_CACHE, v_cache=ONE_CACHE)),
+    (ValueError, "of their own", eight(k_scale=ONE_SCALE, v_scale=ONE_SCALE)),
     (ValueError, "seq_lens", dict(seq_lens=torch.ones(2))),
     (ValueError, "seq_lens", dict(seq_lens=torch.ones(2, 1, dtype=torch.int32))),
     (ValueError, "block_table", dict(block_table=torch.zeros(3, 2, dtype=torch.int32))),

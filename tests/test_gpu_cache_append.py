@@ -66,6 +66,7 @@ CASES = [
     (1, 96, 24, False, 16, "fp8", torch.bfloat16, False),
     (2, 256, 256, False, 300, "fp8", torch.bfloat16, False),   # pages longer than the registers hold
     (2, 32, 0, False, 200, "fp8", torch.float16, False),
+    (5, 64, 32, False, 1, "fp8", torch.bfloat16, False),       # a scale to every token; 5 heads: 4 and 1 to a block
     (2, 27, 10, True, 5, "fp8", torch.bfloat16, False),        # off the vector layout
     (2, 40, 20, False, 7, "fp8", torch.float32, True),
     (3, 20, 12, False, 1, "same", torch.float16, False),

@@ -202,6 +202,25 @@ def test_views_streams_and_repeats(cuda_device):
     assert torch.equal(got[0], want[0]) and torch.equal(got[1], want[1])
 
 
+def test_memory_at_odd_addresses(cuda_device):
+    """Dense tensors that begin off the 16-byte alignment: q, the caches, or both."""
+    dev = cuda_device
+    made = make_case([500, 40], 2, 8, 128, 128, 64, 3, torch.bfloat16, seed=13)
+    q, k, v, ks, vs, table, lens, ids = (x.to(dev) for x in made)
+
+    def shifted(x, by):
+        base = torch.empty(x.numel() + by, dtype=torch.uint8 if x.dtype == FP8 else x.dtype, device=dev)
+        y = base[by:].view(x.dtype) if x.dtype == FP8 else base[by:]
+        y = y.view(x.shape)
+        (y.view(torch.uint8) if x.dtype == FP8 else y).copy_(x.view(torch.uint8) if x.dtype == FP8 else x)
+        return y
+
+    for dq, dk, dv in ((1, 0, 0), (0, 4, 0), (0, 0, 1), (3, 8, 5)):
+        got = m3_sparse_decode(shifted(q, dq), shifted(k, dk), shifted(v, dv), table, lens, ids, return_lse=True,
+                               k_scale=ks, v_scale=vs)
+        check(made, 128, got)
+
+
 def test_two_captured_steps_share_nothing(cuda_device):
     """Two captured graphs replayed on two streams at once, lengths and selections changed in between."""
     dev = cuda_device
