@@ -12,13 +12,15 @@
 //
 // HBM-bound (about one operation per byte): each row is read once, held in registers for the
 // reduction and the rotation, and written once; the backward recomputes r from x (4 flops
-// an element) instead of storing it. What is left to watch is the number of instructions (a warp has some
-// 300 issue slots to the 2 KB it reads and writes in the forward): arithmetic is done two floats at a time, w and the angles
-// are multiplied once for all the heads of a token, addresses advance by a fixed step. Warps stay and walk
-// over their tokens' heads, and hide one another's loads (a second set of registers for the next rows costs
-// more warps than it gains: 243 against 210 us forward). q and k go through one launch, each with blocks of its own. The weights' gradients are summed in
-// registers on the way, then over a block's warps and the blocks in a fixed order (no atomics, the same bits
-// every run).
+// an element) instead of storing it. What is left to watch is the number of instructions: a warp has some 340
+// issue slots to the 2 KB of rows that it reads and writes in the forward. So arithmetic is done two floats at a
+// time, w and the angles are multiplied once for all the heads of a token, and addresses advance by a fixed
+// step. Warps stay and walk over their tokens' heads, and hide one another's loads (a second set of registers for
+// the next rows costs more warps than it gains: 243 against 210 us forward). q and k go through one launch, each
+// with blocks of its own. The weights' gradients are summed in registers on the way, then over a block's warps and
+// the blocks in a fixed order (no atomics, the same bits every run).
+// Measured: 32768 tokens of 64 + 8 heads of 128, bf16: 210 us forward, 5.8 TB/s, 90% of the copy rate; 71168 tokens
+// of 32 + 8 heads: 256 us forward (88%), 407 us backward (5.4 TB/s, 83%).
 #include <algorithm>
 
 #include "rope_common.cuh"
@@ -32,14 +34,14 @@ constexpr int kWarps = 4;
 constexpr int kMaxDimFast = 256;
 constexpr int kMaxDim = 512;
 
-// Rows a lane takes at a time: 64 bytes of loads in flight for every type.
-template <typename T, bool BWD>
-constexpr int kRowsOf = 64 / (2 * kE * (int)sizeof(T)) / (BWD ? 2 : 1);
+// Rows a lane takes at a time: 64 bytes of loads in flight a tensor for every type.
+template <typename T>
+constexpr int kRowsOf = 64 / (2 * kE * (int)sizeof(T));
 
-// Blocks to an SM, by registers (72-76 forward, 96 backward). Measured at 71168 tokens of 40 heads of 128: 6 and 5
-// blocks 256 and 426 us; 7 (spilled) 254 and 465 us; 5 forward 286 us; 4 backward 430 us.
+// Blocks to an SM, by registers (80 forward, 122 backward). Measured at 71168 tokens of 40 heads of 128: forward 256
+// us with 6 blocks, 286 with 5; backward 407 us with 4, 427 with 5 and half the rows at a time, 465 with 7.
 template <bool BWD>
-constexpr int kResident = BWD ? 5 : 6;
+constexpr int kResident = BWD ? 4 : 6;
 
 // One of q and k.
 struct Side {
@@ -210,7 +212,7 @@ __device__ __forceinline__ void fetch(const T* row, int64_t hs, const LaneMap& m
 
 template <typename T, int LPR, bool INTER>
 __global__ void __launch_bounds__(kWarps * 32, kResident<false>) fwd_kernel(const __grid_constant__ Params p) {
-  constexpr int kRows = kRowsOf<T, false>, kSub = 32 / LPR, kSlots = kSub * kRows;
+  constexpr int kRows = kRowsOf<T>, kSub = 32 / LPR, kSlots = kSub * kRows;
   const Side& s = p.side[blockIdx.x >= p.side[1].first_block];
   const int lane = threadIdx.x & 31, l = lane % LPR, sub = lane / LPR;
   const LaneMap m = lane_map<INTER>(l, p.dim, p.rotary);
@@ -273,7 +275,7 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<false>) fwd_kernel(cons
 
 template <typename T, int LPR, bool INTER>
 __global__ void __launch_bounds__(kWarps * 32, kResident<true>) bwd_kernel(const __grid_constant__ Params p) {
-  constexpr int kRows = kRowsOf<T, true>, kSub = 32 / LPR, kSlots = kSub * kRows;
+  constexpr int kRows = kRowsOf<T>, kSub = 32 / LPR, kSlots = kSub * kRows;
   __shared__ __align__(16) float sums[kWarps][kMaxDimFast];
   const Side& s = p.side[blockIdx.x >= p.side[1].first_block];
   const int warp = threadIdx.x >> 5, lane = threadIdx.x & 31, l = lane % LPR, sub = lane / LPR;
@@ -532,7 +534,7 @@ int deal(Params& p, int slots, int most) {
 
 template <typename T, int LPR, bool BWD>
 void launch_rows(Params& p, cudaStream_t st) {
-  const int blocks = deal(p, 32 / LPR * kRowsOf<T, BWD>, kMaxBlocks<BWD>);
+  const int blocks = deal(p, 32 / LPR * kRowsOf<T>, kMaxBlocks<BWD>);
   if constexpr (BWD) {
     if (p.interleaved) bwd_kernel<T, LPR, true><<<blocks, kWarps * 32, 0, st>>>(p);
     else bwd_kernel<T, LPR, false><<<blocks, kWarps * 32, 0, st>>>(p);
