@@ -28,7 +28,7 @@ using namespace rope;
 
 constexpr int kWarps = 8;
 constexpr int kRowsPerLane = 4;
-constexpr int kPageBlocks = 4;  // of the page kernel, to an SM (3: 67 us, 4: 62 us at 32768 tokens of 8 heads of 128)
+constexpr int kPageBlocks = 4;  // of the page kernel, to an SM (3: 67 us, 4: 62)
 constexpr int kMaxDimFast = 256;
 
 struct Half {  // k or v
@@ -274,7 +274,11 @@ __device__ __forceinline__ float block_amax(float v, float* red) {
 // Chunks: a block takes HC heads (4, or 1 of a tensor with fewer) of a (request, page), of k or v. It reads the rows
 // twice, once for the heads' maxima and once for the codes: the second time they come from L2 (a wave of blocks
 // holds some 50 MB, half the L2). That keeps whole kilobytes of a token's heads together and one set of angles for
-// them, and holds nothing on the way. The maximum takes whatever is there: NaN drops out of fmaxf by itself, and
+// them, and holds nothing on the way. (A head at a time to a block, its rows held in registers or copied ahead
+// into shared memory, took 75-93 us: 256-byte pieces two kilobytes apart; eight heads 87: too few blocks.)
+// 32768 tokens, 8 heads of 128 (bf16), pages of 128: 60 us, 3.5 TB/s of the 210 MB that must move, 54% of the copy
+// rate; DRAM reads are 1.1 times the input, so the second pass does hit L2. Issue slots are 66% busy: what is
+// left is instructions (138 a lane for the two passes over a 16-byte piece). The maximum takes whatever is there: NaN drops out of fmaxf by itself, and
 // only a page that holds an infinity is looked through again for its finite values.
 template <typename T, int LPR, bool INTER, int HC>
 __global__ void __launch_bounds__(kWarps * 32, kPageBlocks) append8_page_kernel(const __grid_constant__ Params p) {

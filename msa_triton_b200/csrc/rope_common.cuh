@@ -238,28 +238,26 @@ __device__ __forceinline__ float dot_of(const Lane& x, const Lane& y) {
   return t.x + t.y;
 }
 
-__device__ __forceinline__ F2 add2(F2 a, F2 b) {
-  F2 r;
-  asm("add.rn.f32x2 %0, %1, %2;" : "=l"(r.v) : "l"(a.v), "l"(b.v));
-  return r;
-}
 // A lane's angles, ready for rotate_exact.
 struct Angle2 {
-  F2 c[kE / 2], s[kE / 2], minus[kE / 2];
+  F2 c[kE / 2], s[kE / 2];
   __device__ __forceinline__ void load(const float* cos4, const float* sin4) {
     const float4 x = __ldg(reinterpret_cast<const float4*>(cos4)), y = __ldg(reinterpret_cast<const float4*>(sin4));
     c[0] = pack2(x.x, x.y), c[1] = pack2(x.z, x.w);
     s[0] = pack2(y.x, y.y), s[1] = pack2(y.z, y.w);
-    minus[0] = pack2(-y.x, -y.y), minus[1] = pack2(-y.z, -y.w);
   }
 };
-// rotate_pair, two pairs to an instruction and with its roundings.
+// rotate_pair with its roundings, the products of two pairs to an instruction. The sums are single instructions:
+// a two-float sum of two-float products came out as a fused one although both name their rounding (a few in a
+// million codes differed from rotate_pair's).
 __device__ __forceinline__ void rotate_exact(Lane& x, const Angle2& t) {
 #pragma unroll
   for (int i = 0; i < kE / 2; ++i) {
     const F2 a = x.v[i], b = x.v[kE / 2 + i];
-    x.v[i] = add2(mul2(a, t.c[i]), mul2(b, t.minus[i]));
-    x.v[kE / 2 + i] = add2(mul2(b, t.c[i]), mul2(a, t.s[i]));
+    const float2 ac = unpack2(mul2(a, t.c[i])), bs = unpack2(mul2(b, t.s[i]));
+    const float2 bc = unpack2(mul2(b, t.c[i])), as = unpack2(mul2(a, t.s[i]));
+    x.v[i] = pack2(__fsub_rn(ac.x, bs.x), __fsub_rn(ac.y, bs.y));
+    x.v[kE / 2 + i] = pack2(__fadd_rn(bc.x, as.x), __fadd_rn(bc.y, as.y));
   }
 }
 

@@ -166,6 +166,33 @@ def test_padded_batches_and_bad_pages_write_nothing(cuda_device):
             assert torch.isnan(on[0][int(pool.table[3, 3]), 2].float()).all()  # its key has no angle
 
 
+@pytest.mark.parametrize("inter", [False, True])
+def test_chunks_and_single_tokens_store_the_same_bits(inter, cuda_device):
+    """The same tokens in one packed call and one at a time, the largest of a page first (so that no page moves
+    to a larger scale): 4 million values, enough for a product and a sum rounded as one to show."""
+    dev = cuda_device
+    gen = torch.Generator(device=dev).manual_seed(12)
+    pages, size, heads, dim = 256, 16, 8, 128  # a page to a request
+    k = torch.randn(pages, size, heads, dim, generator=gen, device=dev).bfloat16()
+    k[:, 0] = 10
+    table = m3_rope_table(size, dim, device=dev) * 0.7
+    table[0] = torch.cat((torch.ones(dim // 2), torch.zeros(dim // 2))).to(dev)
+    own = torch.randperm(pages, generator=gen, device=dev).to(torch.int32).view(-1, 1)
+
+    def cache():
+        return torch.zeros(pages, size, heads, dim, dtype=FP8, device=dev), torch.zeros(pages, heads, device=dev)
+
+    (chunk, chunk_scale), (token, token_scale) = cache(), cache()
+    m3_cache_append(k.flatten(0, 1), None, chunk, None, own, torch.full((pages,), size, dtype=torch.int32, device=dev),
+                    cu_seqlens=torch.arange(0, pages * size + 1, size, dtype=torch.int32, device=dev), rope_table=table,
+                    interleaved=inter, k_scale=chunk_scale)
+    for row in range(size):
+        m3_cache_append(k[:, row], None, token, None, own, torch.full((pages,), row + 1, dtype=torch.int32, device=dev),
+                        rope_table=table, interleaved=inter, k_scale=token_scale)
+    assert torch.equal(chunk_scale, token_scale)
+    assert torch.equal(chunk.view(torch.uint8), token.view(torch.uint8))
+
+
 def test_more_new_rows_than_tokens_stores_the_last(cuda_device):
     gen = torch.Generator().manual_seed(5)
     dev = cuda_device
