@@ -71,8 +71,8 @@ def m3_cache_append(
     ``seq_lens[B]`` (int32) counts each request's tokens with the new ones; request b's new
     rows are ``cu_seqlens[b] .. cu_seqlens[b+1] - 1`` (int32 ``[B + 1]``, on the device, not read
     by the host), or row b without ``cu_seqlens`` (``T = B``), and take its last positions.
-    ``rope_table`` rotates the keys as ``m3_qk_norm_rope`` does; without it they are stored as
-    they are. Caches ``[P,S,G,D]`` are written in place; ``k_scale`` / ``v_scale`` come with 8-bit
+    ``rope_table`` rotates the keys as ``m3_qk_norm_rope`` does (NaN where a position lies outside
+    it); without it, or with one of width 0, they are stored as they are. Caches ``[P,S,G,D]`` are written in place; ``k_scale`` / ``v_scale`` come with 8-bit
     ones. Skipped, with nothing written: rows behind ``cu_seqlens[B]``, requests of length 0 (a
     padded batch), pages past the block table's width or outside the cache. A page that receives
     tokens must belong to one request.

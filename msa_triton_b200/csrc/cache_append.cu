@@ -560,9 +560,10 @@ extern "C" int msa_cache_append(const void* k, const void* v, int dtype, int64_t
   MSA_CHECK_ARG(rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim && table_rows >= 0 &&
                     (rotary_dim == 0 || rope_table),
                 "msa_cache_append: rotary_dim must be even and at most head_dim");
+  if (batch == 0 || total_tokens == 0 || max_pages == 0 || num_pages == 0) return MSA_OK;  // empty tensors have no address
+  MSA_CHECK_ARG(k && k_cache && block_table && seq_lens && !v == !v_cache,
+                "msa_cache_append: missing pointers, or v without v_cache");
   MSA_CHECK_ARG(!quantised || (k_scale && (!v || v_scale)), "msa_cache_append: an e4m3 cache needs its scales");
-  MSA_CHECK_ARG(!v == !v_cache, "msa_cache_append: v and v_cache go together");
-  if (batch == 0 || total_tokens == 0 || max_pages == 0 || num_pages == 0) return MSA_OK;
   Params p{};
   p.half[0] = Half{k, k_cache, quantised ? k_scale : nullptr, k_token_stride, k_head_stride,
                    k_page_stride, k_slot_stride, k_cache_head_stride, rotary_dim};

@@ -27,11 +27,11 @@ def encode(x, scale):
 def rotated_f32(k, table, positions, interleaved):
     """The rotation in float32, every product and sum rounded by itself."""
     y = k.float().clone()
-    if table is None:
+    if table is None or table.shape[1] == 0:
         return y
     inside = (positions >= 0) & (positions < table.shape[0])
     cs = table[torch.where(inside, positions, 0)]
-    cos, sin = cs.split(table.shape[1] // 2, -1) if table.shape[1] else (cs, cs)
+    cos, sin = cs.split(table.shape[1] // 2, -1)
     y = R.rotate(y, cos, sin, interleaved)
     y[~inside] = math.nan
     return y

@@ -161,9 +161,16 @@ def test_library_checks_its_arguments():
     with pytest.raises(_lib.MsaError, match="bad dtype"):
         _lib.call("msa_cache_append", n, n, 3, 0, 0, 0, 0, n, 0, 0, 0, n, n, n, 0, 0, 1, 1, 1, 0, 0, n, n, 3, 0, 0, 0, 0,
                   0, 0, n, n, n)
+    some = 16  # never read: the checks come first
     with pytest.raises(_lib.MsaError, match="needs its scales"):
-        _lib.call("msa_cache_append", n, n, 2, 0, 0, 0, 0, n, 0, 0, 0, n, n, n, 0, 0, 1, 1, 1, 0, 0, n, n, 3, 0, 0, 0, 0,
-                  0, 0, n, n, n)
+        _lib.call("msa_cache_append", some, n, 2, 0, 0, 0, 0, n, 0, 0, 0, n, some, some, 1, 1, 1, 1, 1, 1, 1, some, n, 3,
+                  0, 0, 0, 0, 0, 0, n, n, n)
+    with pytest.raises(_lib.MsaError, match="missing pointers"):
+        _lib.call("msa_cache_append", some, some, 2, 0, 0, 0, 0, n, 0, 0, 0, n, some, some, 1, 1, 1, 1, 1, 1, 1, some, n,
+                  2, 0, 0, 0, 0, 0, 0, n, n, n)
+    # nothing to do: no pointer is needed
+    _lib.call("msa_cache_append", n, n, 2, 0, 0, 0, 0, n, 0, 0, 0, n, n, n, 0, 0, 1, 1, 1, 0, 0, n, n, 3, 0, 0, 0, 0, 0, 0,
+              n, n, n)
     with pytest.raises(_lib.MsaError, match="head_dim"):
         _lib.call("msa_decode_attn_e4m3", n, 2, n, n, 0, 0, 0, 0, 0, 0, n, n, n, n, n, 1, 4, 2, 300, 16, 1, 1, 1, 16, 1.0,
                   n, n, n)

@@ -193,6 +193,25 @@ def test_chunks_and_single_tokens_store_the_same_bits(inter, cuda_device):
     assert torch.equal(chunk.view(torch.uint8), token.view(torch.uint8))
 
 
+def test_empty_calls_do_nothing(cuda_device):
+    """No tokens, no requests, no pages: nothing to store, and no error."""
+    dev = cuda_device
+    for kind in (FP8, torch.bfloat16):
+        cache = [torch.zeros(3, 16, 2, 64, device=dev).to(kind) for _ in range(2)]
+        scale = [torch.ones(3, 2, device=dev) if kind == FP8 else None for _ in range(2)]
+        lens = torch.zeros(2, dtype=torch.int32, device=dev)
+        pages, cu = torch.zeros(2, 1, dtype=torch.int32, device=dev), torch.zeros(3, dtype=torch.int32, device=dev)
+        none = torch.zeros(0, 2, 64, dtype=torch.bfloat16, device=dev)
+        m3_cache_append(none, none, *cache, pages, lens, cu_seqlens=cu, k_scale=scale[0], v_scale=scale[1])
+        m3_cache_append(none, none, *cache, pages[:0], lens[:0], k_scale=scale[0], v_scale=scale[1])
+        one = torch.ones(2, 2, 64, dtype=torch.bfloat16, device=dev)
+        m3_cache_append(one, one, *cache, pages[:, :0], lens + 1, k_scale=scale[0], v_scale=scale[1])
+        empty = [c[:0] for c in cache]
+        m3_cache_append(one, one, *empty, pages, lens + 1, k_scale=None if kind != FP8 else scale[0][:0],
+                        v_scale=None if kind != FP8 else scale[1][:0])
+        assert all(torch.count_nonzero(c.float()) == 0 for c in cache)
+
+
 def test_more_new_rows_than_tokens_stores_the_last(cuda_device):
     gen = torch.Generator().manual_seed(5)
     dev = cuda_device

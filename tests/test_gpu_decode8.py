@@ -5,8 +5,10 @@ that the oracle returns:
   * a logit (natural units): D products and sums, q's and the scales' factors, the softmax's subtraction:
     (D + 32) u of its absolute terms; elements of q far below the head's largest are kept to 2^-25 of
     that one (counted in the terms);
-  * a weight: the logit's error twice (numerator and sum), exp2's 2 ulp, one rounding to fp16 (2^-12, or
-    2^-22 for the two-term float32 form), and 2^-25 of the largest weight below fp16's normal range;
+  * a weight: the logit's error twice (numerator and sum), exp2's 2 ulp, one rounding to fp16 (half of its
+    relative step 2^-10, so 2^-11: an 11-bit significand 1.xxxxxxxxxx is off by at most 2^-11 of a number in [1, 2);
+    the two-term float32 form rounds a rest of at most 2^-11 once more, 2^-22), and 2^-25 of the largest weight
+    below fp16's normal range;
   * sums over the keys: one u per key, and the merges (64);
   * the output's own rounding, half a step."""
 
@@ -85,7 +87,7 @@ def check(case, block, got, scale=None):
     assert got[0].dtype == dtype and got[1].dtype == torch.float32
     assert torch.equal(torch.isneginf(got_lse), torch.isneginf(lse))
     logit = (dim + 32) * R.U * size_s
-    weight = 2 * logit + 2.0 ** -21 + (2.0 ** -22 if dtype == torch.float32 else 2.0 ** -12) + (keys + 64) * R.U
+    weight = 2 * logit + 2.0 ** -21 + (2.0 ** -22 if dtype == torch.float32 else 2.0 ** -11) + (keys + 64) * R.U
     bound = (R.half_step(dtype) * out.abs() * (1 + 2.0 ** -6) + weight[..., None] * size_o
              + 2.0 ** -25 * size_w[..., None] + 2.0 ** -25 * (dtype == torch.float16))
     over = (got_out - out).abs() - bound
