@@ -189,3 +189,22 @@ def test_oracle_gradients_match_autograd():
         fx, fw, _, _ = R.norm_rope_backward(x.detach(), w.detach(), g, cos, sin, 1e-3, interleaved)
         torch.testing.assert_close(fx, dx, rtol=1e-11, atol=1e-11)
         torch.testing.assert_close(fw, dw, rtol=1e-11, atol=1e-11)
+
+
+def test_fake_kernels_give_output_shapes():
+    from torch._subclasses.fake_tensor import FakeTensorMode
+
+    import msa_triton_b200.library  # noqa: F401  (registers the operators)
+
+    ops = torch.ops.msa_b200
+    with FakeTensorMode():
+        row = torch.empty(7, 40 * 128, dtype=torch.bfloat16, device="cuda")
+        q, k = row[:, :32 * 128].view(7, 32, 128), row[:, 32 * 128:].view(7, 8, 128)
+        w = torch.empty(128, dtype=torch.float32, device="cuda")
+        table = torch.empty(9, 64, dtype=torch.float32, device="cuda")
+        cu = torch.empty(2, dtype=torch.int32, device="cuda")
+        out = ops.qk_norm_rope(q, k, w, w, table, None, cu, 1e-6, False)
+        assert [x.shape for x in out] == [q.shape, k.shape] and all(x.is_contiguous() for x in out)
+        grads = ops.qk_norm_rope_backward(q, k, w, w, table, None, cu, 1e-6, False, *out, [True, False, True, False])
+        assert grads[0].shape == q.shape and grads[1].numel() == 0 and grads[2].shape == w.shape
+        assert grads[2].dtype == torch.float32 and grads[3].numel() == 0

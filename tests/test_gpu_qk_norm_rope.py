@@ -271,3 +271,14 @@ def test_compiled_call_matches_eager(cuda_device):
     g = (gq.to(dev), gk.to(dev))
     for a, b in zip(torch.autograd.grad(got, leaves, g), torch.autograd.grad(want, leaves, g)):
         assert torch.equal(a, b)
+
+
+def test_registered_operator_passes_opcheck(cuda_device):
+    import msa_triton_b200.library  # noqa: F401  (registers the operators)
+
+    dev = cuda_device
+    lens = [9, 4]
+    q, k, wq, wk, _, _, table = make(lens, 4, 2, 64, 32, torch.float32, torch.float32)
+    leaves = [x.to(dev).requires_grad_() for x in (q, k, wq, wk)]
+    args = (*leaves, table.to(dev), None, cu_of(lens, dev), 1e-6, False)
+    torch.library.opcheck(torch.ops.msa_b200.qk_norm_rope.default, args)
