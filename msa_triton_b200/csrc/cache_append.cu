@@ -10,7 +10,7 @@
 // Two kinds of cache:
 //   * the inputs' type: rotate, round once, store; a warp per (token, heads), HBM-bound;
 //   * e4m3 with a scale per (page, head) (e4m3.cuh). The scale needs the page's maximum before its first
-//     code, so the unit of work is a (request, page, head) of k or v. A page whose first row is among the
+//     code, so the unit of work is a request's page, some heads of k or v. A page whose first row is among the
 //     new ones gets a fresh scale; another keeps its own unless the new rows need more, and then its
 //     earlier rows move to the larger scale. Rows behind the last token are left alone.
 //
@@ -274,12 +274,13 @@ __device__ __forceinline__ float block_amax(float v, float* red) {
 // Chunks: a block takes HC heads (4, or 1 of a tensor with fewer) of a (request, page), of k or v. It reads the rows
 // twice, once for the heads' maxima and once for the codes: the second time they come from L2 (a wave of blocks
 // holds some 50 MB, half the L2). That keeps whole kilobytes of a token's heads together and one set of angles for
-// them, and holds nothing on the way. (A head at a time to a block, its rows held in registers or copied ahead
-// into shared memory, took 75-93 us: 256-byte pieces two kilobytes apart; eight heads 87: too few blocks.)
-// 32768 tokens, 8 heads of 128 (bf16), pages of 128: 60 us, 3.5 TB/s of the 210 MB that must move, 54% of the copy
-// rate; DRAM reads are 1.1 times the input, so the second pass does hit L2. Issue slots are 66% busy: what is
-// left is instructions (138 a lane for the two passes over a 16-byte piece). The maximum takes whatever is there: NaN drops out of fmaxf by itself, and
+// them, and holds nothing on the way. The maximum takes whatever is there: NaN drops out of fmaxf by itself, and
 // only a page that holds an infinity is looked through again for its finite values.
+// Measured: 32768 tokens, 8 heads of 128 (bf16), pages of 128: 60 us, 3.5 TB/s of the 210 MB that must move, 54% of
+// the copy rate; DRAM reads are 1.1 times the input, so the second pass does hit L2. Issue slots are 66% busy:
+// what is left is instructions (138 a lane for the two passes over a 16-byte piece). A head at a time to a
+// block, its rows held in registers or copied ahead into shared memory, took 75-93 us (256-byte pieces two
+// kilobytes apart); eight heads 87 us (too few blocks).
 template <typename T, int LPR, bool INTER, int HC>
 __global__ void __launch_bounds__(kWarps * 32, kPageBlocks) append8_page_kernel(const __grid_constant__ Params p) {
   constexpr int kRows = kWarps * 32 / LPR;  // tokens of a step
@@ -560,7 +561,8 @@ extern "C" int msa_cache_append(const void* k, const void* v, int dtype, int64_t
   MSA_CHECK_ARG(rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim && table_rows >= 0 &&
                     (rotary_dim == 0 || rope_table),
                 "msa_cache_append: rotary_dim must be even and at most head_dim");
-  if (batch == 0 || total_tokens == 0 || max_pages == 0 || num_pages == 0) return MSA_OK;  // empty tensors have no address
+  // nothing to store; empty tensors have no address
+  if (batch == 0 || total_tokens == 0 || max_pages == 0 || num_pages == 0) return MSA_OK;
   MSA_CHECK_ARG(k && k_cache && block_table && seq_lens && !v == !v_cache,
                 "msa_cache_append: missing pointers, or v without v_cache");
   MSA_CHECK_ARG(!quantised || (k_scale && (!v || v_scale)), "msa_cache_append: an e4m3 cache needs its scales");

@@ -118,7 +118,10 @@ __device__ __forceinline__ void cp_async_wait() {
 
 __device__ __forceinline__ uint4 lds128(uint32_t at) {
   uint4 u;
-  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];" : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w) : "r"(at) : "memory");
+  asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+               : "=r"(u.x), "=r"(u.y), "=r"(u.z), "=r"(u.w)
+               : "r"(at)
+               : "memory");
   return u;
 }
 __device__ __forceinline__ uint2 lds64(uint32_t at) {
@@ -195,7 +198,8 @@ __device__ __forceinline__ void store_out(void* out, int64_t row, int d, int dim
     }
 }
 
-// 2^x and log2 x by the special function unit (2 ulp; subnormal results are zero: a weight 2^-126 of the largest).
+// 2^x and log2 x by the special function unit (2 ulp; a subnormal result, a weight 2^-126 of the largest, is
+// zero).
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
@@ -228,7 +232,9 @@ __device__ __forceinline__ void store_cluster4(uint32_t at, float4 x) {
   asm volatile("st.shared::cluster.v4.f32 [%0], {%1, %2, %3, %4};" ::"r"(at), "f"(x.x), "f"(x.y), "f"(x.z), "f"(x.w)
                : "memory");
 }
-__device__ __forceinline__ void cluster_arrive() { asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory"); }
+__device__ __forceinline__ void cluster_arrive() {
+  asm volatile("barrier.cluster.arrive.release.aligned;" ::: "memory");
+}
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
 // Bytes of a warp's shared memory: its ring (keys, values, their scales, the mask of each tile), its list
@@ -253,8 +259,8 @@ __device__ __forceinline__ int part_at(int row, int i) {
 }
 
 // DP: head dim rounded up to 64, 128 or 256. HR: tiles of 8 heads (1 or 2).
-// SPLIT: float32 inputs. VEC: rows (q's and out's too) are 16-byte aligned and dim is a multiple of 16 (other shapes all run the
-// 16-row float32 form, which is right for every type and head count).
+// SPLIT: float32 inputs. VEC: rows (q's and out's too) are 16-byte aligned and dim is a multiple of 16 (other
+// shapes all run the 16-row float32 form, which is right for every type and head count).
 template <int DP, int HR, bool SPLIT, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32, DP == 128 && HR == 1 && !SPLIT ? 3 : 1)
 decode8_kernel(const __grid_constant__ Params p) {
@@ -454,7 +460,10 @@ decode8_kernel(const __grid_constant__ Params p) {
 #pragma unroll
             for (int r = 0; r < HR; ++r) {
               mma(x[kt][r], a0, a1, a2, a3, qa[r][s][0], qa[r][s][1]);
-              if (SPLIT) mma(x[kt][r], a0, a1, a2, a3, qb[SPLIT ? r : 0][SPLIT ? s : 0][0], qb[SPLIT ? r : 0][SPLIT ? s : 0][1]);
+              if (SPLIT) {
+                const uint32_t(&rest)[2] = qb[SPLIT ? r : 0][SPLIT ? s : 0];
+                mma(x[kt][r], a0, a1, a2, a3, rest[0], rest[1]);
+              }
             }
           }
         }
@@ -780,7 +789,8 @@ extern "C" int msa_decode_attn_e4m3(const void* q, int dtype, const void* k_cach
   const bool vec = head_dim % 16 == 0 && reinterpret_cast<uintptr_t>(q) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(out) % 16 == 0 && reinterpret_cast<uintptr_t>(k_cache) % 16 == 0 &&
                    reinterpret_cast<uintptr_t>(v_cache) % 16 == 0 &&
-                   (k_page_stride | k_slot_stride | k_head_stride | v_page_stride | v_slot_stride | v_head_stride) % 16 == 0;
+                   (k_page_stride | k_slot_stride | k_head_stride) % 16 == 0 &&
+                   (v_page_stride | v_slot_stride | v_head_stride) % 16 == 0;
   cudaStream_t st = as_stream(stream);
   const bool few = q_heads / groups <= 8;
   if (head_dim <= 64) return few ? launch_dim<64, 1>(p, batch, vec, st) : launch_dim<64, 2>(p, batch, vec, st);

@@ -31,7 +31,7 @@ from ._lib import DTYPE_CODE, call, device_of, ptr, stream_of
 def _check_paged(block_table, seq_lens, batch, device):
     if block_table.ndim != 2 or block_table.shape[0] != batch or block_table.dtype != torch.int32:
         raise ValueError("block_table must be int32 [B, max_pages]")
-    if seq_lens.ndim != 1 or seq_lens.shape[0] != batch or seq_lens.dtype != torch.int32:
+    if seq_lens.shape != (batch,) or seq_lens.dtype != torch.int32:
         raise ValueError("seq_lens must be int32 [B]")
     if block_table.device != device or seq_lens.device != device:
         raise ValueError("All inputs must reside on the same device.")
@@ -97,11 +97,11 @@ def dense_rows(x: torch.Tensor) -> torch.Tensor:
     return x if x.stride(-1) == 1 or x.shape[-1] == 1 else x.contiguous()
 
 
-def check_scale(name, scale, cache):
+def check_scale(name, scale, pages, groups, device):
     """The scales of an 8-bit cache ``[P, S, G, D]``: float32 ``[P, G]``, dense."""
-    if scale is None or scale.shape != (cache.shape[0], cache.shape[2]) or scale.dtype != torch.float32:
+    if scale is None or scale.shape != (pages, groups) or scale.dtype != torch.float32:
         raise ValueError(f"{name} must be float32 [P,G] for an 8-bit cache")
-    if scale.device != cache.device:
+    if scale.device != device:
         raise ValueError("All inputs must reside on the same device.")
     if not scale.is_contiguous():
         raise ValueError(f"{name} must be contiguous")
@@ -125,8 +125,8 @@ def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, blo
             not (quantised or k_cache.dtype == q.dtype):
         raise TypeError("q/k/v must share a BF16, FP16, or FP32 dtype.")
     if quantised:
-        check_scale("k_scale", k_scale, k_cache)
-        check_scale("v_scale", v_scale, v_cache)
+        check_scale("k_scale", k_scale, k_cache.shape[0], groups, k_cache.device)
+        check_scale("v_scale", v_scale, k_cache.shape[0], groups, v_cache.device)
     elif k_scale is not None or v_scale is not None:
         raise ValueError("k_scale and v_scale belong to an 8-bit cache")
     if indices.ndim != 3 or indices.shape[:2] != (batch, groups) or indices.dtype != torch.int32:
@@ -163,11 +163,11 @@ def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, blo
 def _sparse_decode8(q, k_cache, v_cache, block_table, seq_lens, indices, block_size, scale, return_lse, k_scale,
                     v_scale):
     batch, hq, dim = q.shape
-    out = torch.empty_like(q, memory_format=torch.contiguous_format)
-    lse = torch.empty((batch, hq), dtype=torch.float32, device=q.device)
+    q = q.contiguous()
+    out, lse = torch.empty_like(q), k_scale.new_empty((batch, hq))
     if batch and dim:
         # every copy is held by name until the launch: a temporary's memory would be handed to the next one
-        q, k_cache, v_cache = q.contiguous(), dense_rows(k_cache), dense_rows(v_cache)
+        k_cache, v_cache = dense_rows(k_cache), dense_rows(v_cache)
         block_table, seq_lens, indices = block_table.contiguous(), seq_lens.contiguous(), indices.contiguous()
         pages, page_size, groups, _ = k_cache.shape
         with device_of(q):

@@ -58,11 +58,11 @@ def check_table(rope_table, head_dim, device):
 
 
 def _common(q, k, q_weight, k_weight, table, positions, cu, interleaved):
-    """The arguments that both launchers pass between the tensors and the strides."""
-    nseq = 0 if cu is None else cu.numel() - 1
-    return (DTYPE_CODE[q.dtype], q_weight.data_ptr(), k_weight.data_ptr(), DTYPE_CODE[q_weight.dtype],
-            table.data_ptr(), *table.shape, interleaved, ptr(positions), ptr(cu), nseq, q.shape[0], q.shape[1],
-            k.shape[1], q.shape[2], *q.stride()[:2], *k.stride()[:2])
+    """The arguments that both launchers pass between the tensors and the gradients' strides."""
+    dtype, (total, q_heads, dim), q_strides, k_strides = q.dtype, q.shape, q.stride(), k.stride()
+    return (DTYPE_CODE[dtype], q_weight.data_ptr(), k_weight.data_ptr(), DTYPE_CODE[q_weight.dtype],
+            table.data_ptr(), *table.shape, interleaved, ptr(positions), ptr(cu), 0 if cu is None else cu.shape[0] - 1,
+            total, q_heads, k.shape[1], dim, q_strides[0], q_strides[1], k_strides[0], k_strides[1])
 
 
 def _laid_out(q, k, q_weight, k_weight, table, positions, cu):
@@ -73,7 +73,8 @@ def _laid_out(q, k, q_weight, k_weight, table, positions, cu):
 def norm_rope_forward(q, k, q_weight, k_weight, table, positions, cu, eps, interleaved):
     """(q_out, k_out); shared by the autograd Function and the torch.library operator."""
     q, k, q_weight, k_weight, table, positions, cu = _laid_out(q, k, q_weight, k_weight, table, positions, cu)
-    q_out, k_out = (torch.empty_like(x, memory_format=torch.contiguous_format) for x in (q, k))
+    q_out = torch.empty_like(q, memory_format=torch.contiguous_format)
+    k_out = torch.empty_like(k, memory_format=torch.contiguous_format)
     with device_of(q):
         call("msa_qk_norm_rope_fwd", q.data_ptr(), k.data_ptr(), *_common(q, k, q_weight, k_weight, table, positions, cu,
                                                               interleaved),
@@ -140,31 +141,31 @@ def m3_qk_norm_rope(
     """
     if q.ndim != 3 or k.ndim != 3 or q.shape[0] != k.shape[0] or q.shape[2] != k.shape[2]:
         raise ValueError("expected q[T,Hq,D] and k[T,Hk,D] with matching T and D")
-    dim = q.shape[2]
-    if q.shape[1] <= 0 or k.shape[1] <= 0 or not 0 < dim <= MAX_HEAD_DIM:
+    (total, heads, dim), dtype, device = q.shape, q.dtype, q.device
+    if heads <= 0 or k.shape[1] <= 0 or not 0 < dim <= MAX_HEAD_DIM:
         raise ValueError(f"expected at least one head and a head dimension in [1, {MAX_HEAD_DIM}]")
-    if q.dtype not in (torch.bfloat16, torch.float16, torch.float32) or k.dtype != q.dtype:
+    if dtype not in DTYPE_CODE or k.dtype != dtype:
         raise TypeError("q/k must share a BF16, FP16, or FP32 dtype.")
     if q_weight.shape != (dim,) or k_weight.shape != (dim,):
         raise ValueError("q_weight and k_weight must have shape [D]")
-    if q_weight.dtype not in (q.dtype, torch.float32) or k_weight.dtype != q_weight.dtype:
+    if q_weight.dtype not in (dtype, torch.float32) or k_weight.dtype != q_weight.dtype:
         raise TypeError("the weights must share the inputs' dtype or FP32")
-    check_table(rope_table, dim, q.device)
+    check_table(rope_table, dim, device)
     if (cu_seqlens is None) == (positions is None):
         raise ValueError("give either cu_seqlens or positions")
-    if k.device != q.device or q_weight.device != q.device or k_weight.device != q.device:
+    if k.device != device or q_weight.device != device or k_weight.device != device:
         raise ValueError("All inputs must reside on the same device.")
     if not (math.isfinite(eps) and eps >= 0):
         raise ValueError("eps must be finite and nonnegative")
     if positions is not None:
-        if positions.shape != (q.shape[0],) or positions.dtype != torch.int32:
+        if positions.shape != (total,) or positions.dtype != torch.int32:
             raise ValueError("positions must be int32 [T]")
-        if positions.device != q.device:
+        if positions.device != device:
             raise ValueError("All inputs must reside on the same device.")
     else:
-        if cu_seqlens.device != q.device:
+        if cu_seqlens.device != device:
             raise ValueError("All inputs must reside on the same device.")
-        if max(sequence_lengths(cu_seqlens, q.shape[0], prepared)) > rope_table.shape[0]:
+        if max(sequence_lengths(cu_seqlens, total, prepared)) > rope_table.shape[0]:
             raise ValueError("rope_table has fewer rows than the longest sequence")
     _lib.require_cuda(q)
     if torch.compiler.is_compiling():  # traced by torch.compile: the registered operator

@@ -63,7 +63,8 @@ def append(k, v, k_cache, v_cache, block_table, seq_lens, cu, table, interleaved
                     continue
                 for h in range(x.shape[1]):
                     part = y[here][:, h]
-                    need = power_of_two_scale(float(part[torch.isfinite(part)].abs().max()) if torch.isfinite(part).any() else 0.0)
+                    finite = part[torch.isfinite(part)].abs()
+                    need = power_of_two_scale(float(finite.max()) if len(finite) else 0.0)
                     old = float(scale[page, h])
                     now = need if int(at[0]) == 0 else max(old, need)
                     if int(at[0]) and now > old:

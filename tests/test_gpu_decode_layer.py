@@ -116,8 +116,8 @@ def test_training_layer_gradients_reach_the_projections(cuda_device):
     q, k, v = draw(360, HQ, D), draw(360, G, D), draw(360, G, D)
     wq, wk = 1 + 0.1 * draw(D), 1 + 0.1 * draw(D)
     table = m3_rope_table(300, 64, device=dev)
-    iq, ik = m3_qk_norm_rope(draw(360, G, DI), draw(360, 1, DI), *(torch.ones(DI, dtype=torch.bfloat16, device=dev),) * 2,
-                             table[:, :32].contiguous(), cu)
+    one = torch.ones(DI, dtype=torch.bfloat16, device=dev)
+    iq, ik = m3_qk_norm_rope(draw(360, G, DI), draw(360, 1, DI), one, one, table[:, :32].contiguous(), cu)
     ids = m3_topk(m3_index_score(iq, ik, cu, 260), cu, topk_blocks=2)
     leaves = [x.requires_grad_() for x in (q, k, v, wq, wk)]
     go = draw(360, HQ, D)
