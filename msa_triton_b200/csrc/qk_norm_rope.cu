@@ -109,7 +109,7 @@ __device__ __forceinline__ float row_sum(float x) {
 // ------------------------------------------------------------------ rows in the lane layout
 // A lane's angles of one position, kE cosines and sines; lanes behind the rotated elements: 1 and 0.
 struct Angles {
-  float c[kE], s[kE];
+  float c[kE] = {1.f, 1.f, 1.f, 1.f}, s[kE] = {};
   bool inside = true;
   __device__ __forceinline__ void load(const Params& p, Positions& positions, const LaneMap& m, int64_t t, int l) {
     const int64_t pos = positions.of(p, t);
@@ -224,20 +224,26 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<false>) fwd_kernel(cons
   if (s.flat) {
     const uint32_t rows = (uint32_t)p.tokens * s.heads;
     for (uint32_t item = first; item < s.items; item += stride) {
+      Raw<T> raw[kRows][2];
+      uint32_t token[kRows];
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
         const uint32_t row = item * kSlots + i * kSub + sub, t = row / (uint32_t)s.heads;
-        const bool ok = row < rows && m.active;
-        Raw<T> raw[2];
-        raw[0].u = raw[1].u = {};
-        Angles angles;
-        if (ok) {
+        token[i] = t;
+        raw[i][0].u = raw[i][1].u = {};
+        if (row < rows && m.active) {
           const T* x = static_cast<const T*>(s.x) + t * s.x_ts + (row - t * s.heads) * s.x_hs;
-          raw[0] = load_run(x + m.a), raw[1] = load_run(x + m.b);
-          angles.load(p, positions, m, t, l);
+          raw[i][0] = load_run(x + m.a), raw[i][1] = load_run(x + m.b);
         }
+      }
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const uint32_t row = item * kSlots + i * kSub + sub, t = token[i];
+        const bool ok = row < rows && m.active;
+        Angles angles;
+        if (ok) angles.load(p, positions, m, t, l);
         float f[2 * kE], y[2 * kE];
-        unpack_lane<INTER>(raw, f);
+        unpack_lane<INTER>(raw[i], f);
         fwd_row<LPR, INTER>(p, m, f, w, t, l, angles.inside, Turn(angles, w), y);
         if (ok) store_lane<INTER>(out + (int64_t)row * p.dim + m.a, out + (int64_t)row * p.dim + m.b, y);
       }
@@ -288,24 +294,29 @@ __global__ void __launch_bounds__(kWarps * 32, kResident<true>) bwd_kernel(const
   if (s.flat) {
     const uint32_t rows = (uint32_t)p.tokens * s.heads;
     for (uint32_t item = first; item < s.items; item += stride) {
+      Raw<T> rx[kRows][2], rg[kRows][2];
+      uint32_t token[kRows], last = ~0u;
 #pragma unroll
       for (int i = 0; i < kRows; ++i) {
-        const uint32_t row = item * kSlots + i * kSub + sub, t = row / (uint32_t)s.heads;
-        const bool ok = row < rows && m.active;
-        Raw<T> rx[2], rg[2];
-        rx[0].u = rx[1].u = rg[0].u = rg[1].u = {};
-        Angles angles;
-        if (ok) {
-          const uint32_t h = row - t * s.heads;
+        const uint32_t row = item * kSlots + i * kSub + sub, t = row / (uint32_t)s.heads, h = row - t * s.heads;
+        token[i] = t;
+        rx[i][0].u = rx[i][1].u = rg[i][0].u = rg[i][1].u = {};
+        if (row < rows && m.active) {
           const T* x = static_cast<const T*>(s.x) + t * s.x_ts + h * s.x_hs;
           const T* g = static_cast<const T*>(s.g) + t * s.g_ts + h * s.g_hs;
-          rx[0] = load_run(x + m.a), rx[1] = load_run(x + m.b);
-          rg[0] = load_run(g + m.a), rg[1] = load_run(g + m.b);
-          angles.load(p, positions, m, t, l);
+          rx[i][0] = load_run(x + m.a), rx[i][1] = load_run(x + m.b);
+          rg[i][0] = load_run(g + m.a), rg[i][1] = load_run(g + m.b);
         }
+      }
+      Angles angles;
+#pragma unroll
+      for (int i = 0; i < kRows; ++i) {
+        const uint32_t row = item * kSlots + i * kSub + sub;
+        const bool ok = row < rows && m.active;
+        if (ok && token[i] != last) angles.load(p, positions, m, last = token[i], l);
         float fx[2 * kE], fg[2 * kE], y[2 * kE];
-        unpack_lane<INTER>(rx, fx);
-        unpack_lane<INTER>(rg, fg);
+        unpack_lane<INTER>(rx[i], fx);
+        unpack_lane<INTER>(rg[i], fg);
         bwd_row<LPR>(p, m, lane_of(fx), lane_of(fg), w, angles, ok, dw, y);
         if (ok && out) store_lane<INTER>(out + (int64_t)row * p.dim + m.a, out + (int64_t)row * p.dim + m.b, y);
       }
@@ -510,9 +521,11 @@ int blocks_for(int64_t items, int most) {
   return (int)std::max<int64_t>(1, std::min<int64_t>(most, (items + kWarps - 1) / kWarps));
 }
 
-// Items of both sides, and each side's share of the blocks.
+// Items of both sides, and each side's share of the blocks. A flat step costs more, its angles being loaded row by
+// row: in halves of another step's.
+constexpr int kFlatCost = 3;
 int deal(Params& p, int slots, int most) {
-  int64_t steps[2];
+  int64_t steps[2], cost[2];
   for (int i = 0; i < 2; ++i) {
     Side& s = p.side[i];
     s.flat = s.heads < slots;
@@ -522,8 +535,9 @@ int deal(Params& p, int slots, int most) {
     s.span = (uint32_t)std::max<int64_t>(1, std::min<int64_t>(s.chunks, steps[i] / ((int64_t)most * kWarps * 8)));
     s.spans = ceil_div(s.chunks, s.span);
     s.items = (uint32_t)(s.flat ? steps[i] : p.tokens * s.spans);
+    cost[i] = steps[i] * (s.flat ? kFlatCost : 2);
   }
-  int k_blocks = (int)std::max<int64_t>(1, (most * steps[1] + (steps[0] + steps[1]) / 2) / (steps[0] + steps[1]));
+  int k_blocks = (int)std::max<int64_t>(1, (most * cost[1] + (cost[0] + cost[1]) / 2) / (cost[0] + cost[1]));
   k_blocks = std::min(blocks_for(p.side[1].items, most - 1), k_blocks);
   p.side[0].first_block = 0;
   p.side[0].blocks = blocks_for(p.side[0].items, most - k_blocks);
