@@ -668,6 +668,7 @@ decode8_kernel(const __grid_constant__ Params p) {
   if (splits == 1) return;
 
   // ---- this block's elements, from its own memory: nobody reads it any more after this
+  __syncwarp();  // the cluster barrier takes whole warps
   cluster_arrive();
   cluster_wait();
   const float4* shares = reinterpret_cast<const float4*>(smem + kWarps * L::kBytes);
