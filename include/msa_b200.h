@@ -481,7 +481,8 @@ int msa_qk_norm_rope_bwd(const void* q, const void* k, const void* grad_q, const
  * earlier rows keeps a larger scale or moves them to the new one. Values that are not finite become
  * NaN codes and do not count for the scale. A key whose position lies outside the table is NaN. Rows
  * behind the last request, positions below 0 and pages outside the block table's max_pages or the
- * cache are skipped. A page receives tokens of one request only. */
+ * cache are skipped. A page receives tokens of one request only. page_size * D stays below 2^31, where
+ * head rows are whole aligned vectors below 2^34 (8 bits) or without a bound (the inputs' dtype). */
 int msa_cache_append(const void* k, const void* v, int dtype, int64_t k_token_stride, int64_t k_head_stride,
                      int64_t v_token_stride, int64_t v_head_stride, const float* rope_table, int64_t table_rows,
                      int32_t rotary_dim, int interleaved, const int32_t* cu_seqlens, const int32_t* block_table,

@@ -81,7 +81,8 @@ def m3_cache_append(
     written in place; ``k_scale`` / ``v_scale`` (positive) come with 8-bit ones, whose values that are
     not finite are stored as NaN. Skipped, with nothing written: rows behind ``cu_seqlens[B]``,
     requests of length 0 (a padded batch), pages past the block table's width or outside the cache.
-    A page that receives tokens must belong to one request.
+    A page that receives tokens must belong to one request. Pages of 2^31 elements a head are refused where
+    head rows are not whole aligned vectors, of 2^34 in 8 bits.
     """
     if k.ndim != 3 or (v is not None and v.shape != k.shape):
         raise ValueError("expected k[T,G,D] and a matching v")

@@ -514,7 +514,12 @@ int launch(Params p, int halves, int dtype, bool quantised, cudaStream_t st) {
   const int64_t tasks = p.cu ? p.tokens / p.page_size + 2 * (int64_t)p.batch : p.batch;
   MSA_CHECK_ARG(tasks * p.heads * halves < (int64_t)1 << 31 && p.heads <= 65535,
                 "msa_cache_append: too many pages or heads");
-  if (fast_shape(p, halves, dtype, quantised)) {
+  const bool fast = fast_shape(p, halves, dtype, quantised);
+  // move_rows counts 16-byte units, append_any_kernel elements, of a head's page in 32 bits
+  const int64_t page_elements = (int64_t)p.page_size * p.dim;
+  MSA_CHECK_ARG(page_elements < (int64_t)1 << (!fast ? 31 : quantised ? 34 : 62),
+                "msa_cache_append: page_size * head_dim is too large for this layout");
+  if (fast) {
     const int lpr = p.dim <= 32 ? 4 : p.dim <= 64 ? 8 : p.dim <= 128 ? 16 : 32;
     p.head_chunks = ceil_div(p.heads, 32 / lpr * kRowsPerLane);
     p.chunks = quantised ? halves : p.head_chunks * halves;

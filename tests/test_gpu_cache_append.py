@@ -11,6 +11,7 @@ import pytest
 import torch
 
 from msa_triton_b200 import m3_cache_append, m3_rope_table
+from msa_triton_b200._lib import MsaError
 from tests import cache_oracle as C
 from tests import rope_oracle as R
 
@@ -328,3 +329,22 @@ def test_offsets_past_32_bits(cuda_device):
     same("codes", torch.stack((cache[pages - 5], cache[pages - 1])), small)
     same("scales", scale[[pages - 5, pages - 1]], small_scale)
     assert torch.count_nonzero(cache[:pages - 9].view(torch.uint8)) == 0
+
+
+@pytest.mark.parametrize("kind", [FP8, torch.bfloat16], ids=str)
+def test_pages_past_32_bits(kind, cuda_device):
+    """The last token of a page of 2^31 elements; off the vector layout, where elements are counted in 32 bits, such
+    a page is refused."""
+    dev = cuda_device
+    for dim, size in ((128, 2 ** 24), (100, 2 ** 31 // 100 + 1)):
+        cache = torch.zeros(1, size, 1, dim, dtype=kind, device=dev)
+        scale = torch.ones(1, 1, device=dev) if kind == FP8 else None
+        held = torch.tensor([size], dtype=torch.int32, device=dev)
+        k = torch.randint(-8, 9, (1, 1, dim), device=dev).bfloat16()
+        if dim == 100:
+            with pytest.raises(MsaError, match="too large"):
+                m3_cache_append(k, None, cache, None, held[:, None] * 0, held, k_scale=scale)
+            continue
+        m3_cache_append(k, None, cache, None, held[:, None] * 0, held, k_scale=scale)
+        assert torch.equal(cache[0, -1].float(), k[0].float())
+        assert not cache[0, -3:-1].float().any() and not cache[0, :2].float().any()
