@@ -282,3 +282,34 @@ def test_registered_operator_passes_opcheck(cuda_device):
     leaves = [x.to(dev).requires_grad_() for x in (q, k, wq, wk)]
     args = (*leaves, table.to(dev), None, cu_of(lens, dev), 1e-6, False)
     torch.library.opcheck(torch.ops.msa_b200.qk_norm_rope.default, args)
+
+
+def test_rows_past_32_bit_offsets(cuda_device):
+    """Queries of more than 2^31 elements: rows at both ends, forward and backward, match a short call on them."""
+    dev = cuda_device
+    heads, dim, short = 64, 128, 5
+    total = 2 ** 31 // (heads * dim) + short
+    gen = torch.Generator(device=dev).manual_seed(21)
+    ends = torch.cat((torch.arange(short), torch.arange(total - short, total))).to(dev)
+    q = torch.zeros(total, heads, dim, dtype=torch.bfloat16, device=dev)
+    q[ends] = torch.randn(2 * short, heads, dim, generator=gen, device=dev).bfloat16()
+    k = torch.zeros(total, 1, dim, dtype=torch.bfloat16, device=dev)
+    k[ends] = torch.randn(2 * short, 1, dim, generator=gen, device=dev).bfloat16()
+    wq, wk = ((1 + 0.3 * torch.randn(dim, generator=gen, device=dev)).requires_grad_() for _ in range(2))
+    table = m3_rope_table(64, dim, device=dev)
+    positions = (torch.arange(total, device=dev) % 64).to(torch.int32)
+
+    def run(q, k, positions):
+        q, k = q.requires_grad_(), k.requires_grad_()
+        yq, yk = m3_qk_norm_rope(q, k, wq, wk, table, positions=positions)
+        return yq, yk, *torch.autograd.grad((yq, yk), (q, k, wq, wk), (q.detach(), k.detach()))
+
+    # zero rows add nothing to the weights' gradients
+    want = run(q[ends].clone(), k[ends].clone(), positions[ends])
+    got = run(q, k, positions)
+    for a, b in zip(got[:4], want[:4]):
+        assert torch.equal(a[ends], b)
+        assert torch.count_nonzero(a[short:-short]) == 0
+    for a, b, rows in zip(got[4:], want[4:], (2 * short * heads, 2 * short)):
+        # the same rows in another order: a float32 rounding per row on each side, of |g'| |x'| <= 3 * 6 * 6
+        assert (a - b).abs().max() <= 2 * rows * 2.0 ** -24 * 108 * rows
