@@ -716,22 +716,30 @@ int launch(Params p, int batch, cudaStream_t st) {
     per_sm = std::max(per_sm, 1);
     resident.store(per_sm, std::memory_order_relaxed);
   }
-  // Whole waves of items go a block each, which costs the least in merging; what is over and above them is
-  // split over clusters of the size that finishes first, and goes first, so that the chip is full to the end
-  // (64 requests of 8 groups and 16 blocks: 65.5 us, 67.4 with two blocks to every item; 24 requests of 2
-  // groups, a full wave or less: 11.5 against 16).
+  // Less than a wave of items: each on a cluster of the size that finishes first. More: a block to an item costs the
+  // least in merging, but the blocks behind the last whole wave would run on a chip that is mostly idle. If they are
+  // no more than half a wave, as many items, or a sixth of a wave if that is more, go to pairs of blocks, first: the
+  // lone blocks behind them start at another time than the others, and the pairs' slots take the last ones. Measured
+  // (16 blocks, 8 groups of 128; a wave is 444 items): 64 requests 57.9 us (77.1 with lone blocks alone, 67 with
+  // clusters of 4, 58.4 with pairs for the 68 items over and above the wave alone), 56 requests 55.3 (60.3, 69,
+  // 56.8), 128 requests 103 (114.5, 116, 103); 80 requests, 196 items behind the wave, 73 (79.8); 96, 324 items
+  // behind it: 81.6 alone, 89 with pairs.
   const int64_t head_tiles = ceil_div(p.q_heads / p.groups, 16), items = (int64_t)batch * p.groups;
-  const int64_t slots = std::max<int64_t>(148 * per_sm / head_tiles, 1);
+  const int64_t slots = std::max<int64_t>(148 * per_sm / head_tiles, 1), behind = items % slots;
   const int64_t tiles = (int64_t)p.topk * ((p.block + kTile - 1) / kTile);
-  const int64_t alone = items / slots * slots;
   int64_t shared = 0;
-  double best = 0;
-  for (int shift = 0; (1 << shift) <= kMaxSplits; ++shift) {
-    if (shift && ((int64_t)kWarps << (shift - 1)) >= tiles) break;  // no more warps than tiles
-    const int64_t rest = items - (alone >> shift << shift);           // whole clusters of lone blocks behind them
-    const double waves = (double)(((rest << shift) + slots - 1) / slots);
-    const double cost = waves * ((double)tiles / (kWarps << shift) + kOverhead);
-    if (shift == 0 || cost < best) best = cost, p.split_shift = shift, shared = shift ? rest : 0;
+  if (items < slots) {
+    double best = 0;
+    for (int shift = 0; (1 << shift) <= kMaxSplits; ++shift) {
+      if (shift && ((int64_t)kWarps << (shift - 1)) >= tiles) break;  // no more warps than tiles
+      const double waves = (double)(((items << shift) + slots - 1) / slots);
+      const double cost = waves * ((double)tiles / (kWarps << shift) + kOverhead);
+      if (shift == 0 || cost < best) best = cost, p.split_shift = shift, shared = shift ? items : 0;
+    }
+  } else if (behind > 0 && behind <= slots / 2 && tiles > kWarps) {
+    p.split_shift = 1;
+    shared = std::max(behind, slots / 6);
+    shared += (items - shared) & 1;  // whole clusters of lone blocks
   }
   p.shared = (int)shared;
   cudaLaunchConfig_t cfg{};
