@@ -282,3 +282,17 @@ def test_cache_past_32_bits(cuda_device):
     small = [torch.stack([x[int(i)] for i in at]).cpu() for x in (k_cache, v_cache, *scale)]
     case = (q, *small, torch.arange(8, dtype=torch.int32).view(1, 8), lens, ids)
     check(case, 128, got)
+
+
+@pytest.mark.parametrize("batch,heads,ratio,dim,dtype", [
+    (148, 3, 8, 128, torch.bfloat16), (149, 3, 8, 128, torch.bfloat16), (150, 3, 4, 128, torch.float16),
+    (151, 3, 8, 128, torch.bfloat16), (225, 3, 8, 128, torch.bfloat16), (60, 4, 20, 128, torch.float16),
+    (83, 5, 8, 256, torch.bfloat16), (61, 5, 12, 256, torch.float32), (101, 7, 8, 64, torch.float16)])
+def test_more_requests_than_run_at_once(batch, heads, ratio, dim, dtype, cuda_device):
+    """Around whole waves of blocks and behind them, where the first items are shared between blocks and the others
+    have one each; every tenth request is empty."""
+    gen = torch.Generator().manual_seed(batch)
+    lens = torch.randint(1, 600, (batch,), generator=gen)
+    lens[::10] = 0
+    case = make_case(lens.tolist(), heads, ratio, dim, 128, 64, 4, dtype, seed=batch)
+    check(case, 128, run(case, 128, cuda_device))
