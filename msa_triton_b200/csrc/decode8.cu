@@ -17,10 +17,11 @@
 //     tile t are renumbered to the dims 16 n + 2 t and 16 n + 2 t + 1. P^T's fragment is S^T's after
 //     movmatrix.
 // e4m3 fits fp16 exactly, so the operands are fp16: K and V exact; q divided by a power of two per head
-// (exact but for elements 2^-14 below the head's largest, which keep 2^-25 of it); the weights rounded to
-// 11 bits, an eighth of a bf16 output's own rounding and as much as an fp16 output's (measured error against
-// float64: 1.3 times that of float32 arithmetic rounded once). float32 inputs take both q and the
-// weights as a sum of two fp16 numbers. Accumulators, maxima and sums are float32.
+// (16-bit q exact but for elements 2^-14 below the head's largest, which keep 2^-25 of it; float32 q as a sum of two
+// fp16 numbers); the weights as a sum of two fp16 numbers for every type, 2^-22 of a weight, so that an output's own
+// rounding is the one that shows. (One fp16 number a weight: an fp16 output's error against float64 is 1.3 times
+// that of float32 arithmetic, for 61.3 instead of 62.5 us at 64 requests, 393 instead of 401 us at 256 long ones.)
+// Accumulators, maxima and sums are float32.
 //
 // The values' scales vary by page, so the weights 2^(x_j) vs_j have a running maximum of their own (M' over
 // x_j + log2 vs_j) beside the softmax's M: both stay in fp16's range whatever the scales are.
@@ -259,7 +260,7 @@ __device__ __forceinline__ int part_at(int row, int i) {
 }
 
 // DP: head dim rounded up to 64, 128 or 256. HR: tiles of 8 heads (1 or 2).
-// SPLIT: float32 inputs. VEC: rows (q's and out's too) are 16-byte aligned and dim is a multiple of 16 (other
+// SPLIT: float32 inputs (q in two terms). VEC: rows (q's and out's too) are 16-byte aligned and dim is a multiple of 16 (other
 // shapes all run the 16-row float32 form, which is right for every type and head count).
 template <int DP, int HR, bool SPLIT, bool VEC>
 __global__ void __launch_bounds__(kWarps * 32, DP == 128 && HR == 1 && !SPLIT ? 3 : 1)
@@ -546,7 +547,7 @@ decode8_kernel(const __grid_constant__ Params p) {
       // ---- O^T += V^T P^T
 #pragma unroll
       for (int s = 0; s < kKT; ++s) {
-        uint32_t b[HR][2], rest[SPLIT ? HR : 1][2];
+        uint32_t b[HR][2], rest[HR][2];
 #pragma unroll
         for (int r = 0; r < HR; ++r)
 #pragma unroll
@@ -554,7 +555,7 @@ decode8_kernel(const __grid_constant__ Params p) {
             const float y0 = x[s][r][2 * a], y1 = x[s][r][2 * a + 1];
             const uint32_t packed = pack_half2(y0, y1);
             b[r][a] = transpose8(packed);
-            if (SPLIT) rest[SPLIT ? r : 0][a] = transpose8(pack_rest(y0, y1, packed));
+            rest[r][a] = transpose8(pack_rest(y0, y1, packed));
           }
 #pragma unroll
         for (int c = 0; c < kVC; ++c) {
@@ -573,19 +574,24 @@ decode8_kernel(const __grid_constant__ Params p) {
 #pragma unroll
           for (int w = 0; w < kVB / 4; ++w) {
             // four dims of the keys (2j, 2j + 1) and (2j + 8, 2j + 9): two tiles
+            uint32_t a[2][4];
 #pragma unroll
             for (int half = 0; half < 2; ++half) {
               const uint32_t pick = half ? 0x7362 : 0x5140;
-              uint32_t a0, a1, a2, a3;
-              e4m3::decode4(__byte_perm(vw[0][w], vw[1][w], pick), a0, a1);
-              e4m3::decode4(__byte_perm(vw[2][w], vw[3][w], pick), a2, a3);
-              const int t = c * (kVB / 2) + 2 * w + half;
-#pragma unroll
-              for (int r = 0; r < HR; ++r) {
-                mma(o[r][t], a0, a1, a2, a3, b[r][0], b[r][1]);
-                if (SPLIT) mma(o[r][t], a0, a1, a2, a3, rest[SPLIT ? r : 0][0], rest[SPLIT ? r : 0][1]);
-              }
+              e4m3::decode4(__byte_perm(vw[0][w], vw[1][w], pick), a[half][0], a[half][1]);
+              e4m3::decode4(__byte_perm(vw[2][w], vw[3][w], pick), a[half][2], a[half][3]);
             }
+            // the tiles in turn: the second term of one would wait for its first
+#pragma unroll
+            for (int term = 0; term < 2; ++term)
+#pragma unroll
+              for (int half = 0; half < 2; ++half)
+#pragma unroll
+                for (int r = 0; r < HR; ++r) {
+                  const uint32_t(&weights)[2] = term ? rest[r] : b[r];
+                  mma(o[r][c * (kVB / 2) + 2 * w + half], a[half][0], a[half][1], a[half][2], a[half][3], weights[0],
+                      weights[1]);
+                }
           }
         }
       }

@@ -1,0 +1,41 @@
+"""The softmax weights of the 8-bit decode: inputs whose logits are so small that their errors say little, so
+that the bound is what the weights and the values' scales leave.
+
+Tolerance (u = 2^-24, sizes from the oracle; the bound of test_gpu_decode8.py without a rounding of the weights
+to 16 bits): a logit's error (D + 32) u of its absolute terms, twice; exp2's 2 ulp (2^-21 with the argument's); a weight
+as the sum of two fp16 numbers, 2^-22; one u per key and 64 for the merges; the output's own rounding, half a
+step. ``cut``: what a weight loses at most below fp16's normal range, of its row's largest weight times scale."""
+
+import pytest
+import torch
+
+from tests import cache_oracle as C
+from tests import rope_oracle as R
+from tests.test_gpu_decode8 import make_case, run
+
+pytestmark = pytest.mark.gpu
+FP8 = torch.float8_e4m3fn
+TYPES = [torch.bfloat16, torch.float16, torch.float32]
+
+
+def check(case, block, got, cut, scale=None):
+    q, k, v, ks, vs, table, lens, ids = case
+    dim, dtype = q.shape[2], q.dtype
+    eff = dim ** -0.5 if scale is None else scale
+    out, _, size_s, size_o, size_w, keys = C.attend(q, k, v, ks, vs, table, lens, ids, block, eff)
+    weight = 2 * (dim + 32) * R.U * size_s + 2.0 ** -21 + 2.0 ** -22 + (keys + 64) * R.U
+    bound = (R.half_step(dtype) * out.abs() * (1 + 2.0 ** -6) + weight[..., None] * size_o + cut * size_w[..., None]
+             + 2.0 ** -25 * (dtype == torch.float16))
+    got_out = got[0].cpu().double()
+    assert not torch.isnan(got_out).any()
+    off = (got_out - out).abs()
+    assert float((off - bound).max()) <= 0, f"{float((off / bound.clamp(min=1e-300)).max())} of the bound"
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("ratio,dim", [(8, 128), (16, 128), (4, 64), (3, 27), (8, 256)])
+def test_weights_keep_float32(ratio, dim, dtype, cuda_device):
+    """Few keys with weights close to one another: a weight rounded to the output's bits would show."""
+    made = make_case([3, 5, 9, 17, 40, 70], 2, ratio, dim, 128, 16, 4, dtype, seed=dim + ratio)
+    made[0].mul_(0.02)
+    check(made, 128, run(made, 128, cuda_device), 2.0 ** -25)
