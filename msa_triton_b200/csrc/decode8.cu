@@ -24,7 +24,10 @@
 // Accumulators, maxima and sums are float32.
 //
 // The values' scales vary by page, so the weights 2^(x_j) vs_j have a running maximum of their own (M' over
-// x_j + log2 vs_j) beside the softmax's M: both stay in fp16's range whatever the scales are.
+// x_j + log2 vs_j) beside the softmax's M: no weight leaves fp16's range whatever the scales are. What they lose at
+// its lower end, 2^-25, is lost against a largest weight that stands at 2^14 of fp16's 2^16 (the output is scaled back
+// by 2^-14): at most 2^-39 of the row's largest weight times value scale. Weights up to 1 would lose 2^-25 of it, and
+// the sum of many keys far below the largest with them.
 //
 // A warp works on its own, 32 keys at a time, through a ring of kStages tiles in shared memory that
 // cp.async fills (16 bytes a lane; the 16-byte units of a line are permuted so that neither product's
@@ -43,6 +46,7 @@ constexpr int kWarps = 4;
 constexpr int kTile = 32;      // keys a warp takes at a time
 constexpr int kStages = 2;     // tiles of a warp's ring
 constexpr int kMaxSplits = 8;  // blocks of a cluster
+constexpr int kLift = 14;      // weights relative to the largest times 2^kLift, see below
 
 struct Cache {
   const uint8_t* p;
@@ -534,7 +538,7 @@ decode8_kernel(const __grid_constant__ Params p) {
             for (int e = 0; e < 2; ++e) {
               float& y = x[kt][r][2 * a + e];
               l[r][e] += fast_exp2(y - base[r][e]);
-              y = fast_exp2(y + shift[kt][a] - base_v[r][e]);
+              y = fast_exp2(y + shift[kt][a] - base_v[r][e]) * (1 << kLift);  // not in the exponent: logits may be large
             }
       if (__any_sync(0xffffffffu, rescale)) {
 #pragma unroll
@@ -630,9 +634,11 @@ decode8_kernel(const __grid_constant__ Params p) {
   auto finish = [&](int row, int i, float m, float mv, float sum, float4 acc) {
     // no key: zero and -inf; a NaN sum stays one
     const bool none = m == -INFINITY && sum == 0.f;
-    const float f = none ? 0.f : exp2f((mv == -INFINITY ? 0.f : mv) - (m == -INFINITY ? 0.f : m)) / sum;
+    // the sum and 2^kLift first: the product stays near the codes, whatever the scales are
+    const float f = exp2f((mv == -INFINITY ? 0.f : mv) - (m == -INFINITY ? 0.f : m)), g = 1.f / (1 << kLift) / sum;
     store_out<VEC>(p.out, q_row + row, 4 * i, p.dim, p.dtype,
-                   none ? make_float4(0.f, 0.f, 0.f, 0.f) : make_float4(acc.x * f, acc.y * f, acc.z * f, acc.w * f));
+                   none ? make_float4(0.f, 0.f, 0.f, 0.f)
+                        : make_float4(acc.x * g * f, acc.y * g * f, acc.z * g * f, acc.w * g * f));
     if (i == 0) p.lse[q_row + row] = none ? -INFINITY : ((m == -INFINITY ? 0.f : m) + log2f(sum)) * 0.6931471805599453f;
   };
   auto add = [](float4& acc, const float4& v, float f) {

@@ -39,3 +39,44 @@ def test_weights_keep_float32(ratio, dim, dtype, cuda_device):
     made = make_case([3, 5, 9, 17, 40, 70], 2, ratio, dim, 128, 16, 4, dtype, seed=dim + ratio)
     made[0].mul_(0.02)
     check(made, 128, run(made, 128, cuda_device), 2.0 ** -25)
+
+
+# Half of fp16's smallest step, 2^-25, over a largest weight of 2^13 or more.
+CUT = 2.0 ** -38
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_many_small_weights_beside_a_few_large_ones(dtype, cuda_device):
+    """In every 32 keys one that outweighs the others by e^17.5 and whose value is zero in the odd dims, where the
+    others' values have one sign: what is left of them there is their sum alone."""
+    made = make_case([1100], 1, 4, 64, 128, 128, 9, dtype, seed=1)
+    q, k, v, ks, vs, table, lens, ids = made
+    gen = torch.Generator().manual_seed(2)
+    kc, vc = torch.zeros(k.shape), torch.randint(4, 400, v.shape, generator=gen).float()
+    kc[:, ::32, :, 0] = 7
+    vc[:, ::32, :, 1::2] = 0
+    k.copy_(kc.to(FP8))
+    v.copy_(vc.to(FP8))
+    ks.fill_(1.0)
+    q.zero_()
+    q[..., 0] = 20
+    check(made, 128, run(made, 128, cuda_device), CUT)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+@pytest.mark.parametrize("far", [12, 20])
+def test_pages_with_a_large_value_scale(far, dtype, cuda_device):
+    """Every second page has a value scale 2^far times the others' and zeros in the odd dims."""
+    made = make_case([180, 60], 2, 8, 64, 128, 16, 2, dtype, seed=far)
+    q, k, v, ks, vs, table, lens, ids = made
+    large = torch.zeros(k.shape[0], dtype=torch.bool)
+    large[table[:, ::2].flatten().clamp(min=0).long()] = True
+    bits = v.view(torch.uint8)
+    codes = bits[large]
+    codes[..., 1::2] = 0
+    bits[large] = codes
+    vs.copy_(torch.where(large[:, None], 2.0 ** (far - 8), 2.0 ** -8))
+    q.mul_(0.01)
+    if dtype == torch.float16:
+        vs.mul_(2.0 ** (8 - far))  # within fp16's range
+    check(made, 128, run(made, 128, cuda_device), CUT)
