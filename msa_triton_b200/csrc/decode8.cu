@@ -635,7 +635,8 @@ decode8_kernel(const __grid_constant__ Params p) {
     // no key: zero and -inf; a NaN sum stays one
     const bool none = m == -INFINITY && sum == 0.f;
     // the sum and 2^kLift first: the product stays near the codes, whatever the scales are
-    const float f = exp2f((mv == -INFINITY ? 0.f : mv) - (m == -INFINITY ? 0.f : m)), g = 1.f / (1 << kLift) / sum;
+    // (no value scale above zero: mv is -inf, f 0, and a NaN sum or value stays one)
+    const float f = mv == -INFINITY ? 0.f : exp2f(mv - (m == -INFINITY ? 0.f : m)), g = 1.f / (1 << kLift) / sum;
     store_out<VEC>(p.out, q_row + row, 4 * i, p.dim, p.dtype,
                    none ? make_float4(0.f, 0.f, 0.f, 0.f)
                         : make_float4(acc.x * g * f, acc.y * g * f, acc.z * g * f, acc.w * g * f));

@@ -80,3 +80,16 @@ def test_pages_with_a_large_value_scale(far, dtype, cuda_device):
     if dtype == torch.float16:
         vs.mul_(2.0 ** (8 - far))  # within fp16's range
     check(made, 128, run(made, 128, cuda_device), CUT)
+
+
+@pytest.mark.parametrize("dtype", TYPES)
+def test_no_value_scale_left_far_below_zero(dtype, cuda_device):
+    """Pages of scale 0 stand for zeros: also where every logit is far below zero."""
+    made = make_case([300, 40, 1], 2, 8, 128, 128, 64, 3, dtype, seed=9)
+    q, k, v, ks, vs, *_ = made
+    k.copy_(k.float().abs().to(FP8))
+    q.copy_(-3 * q.abs())
+    vs[:] = 0
+    out, lse = run(made, 128, cuda_device)
+    assert (lse < -100).any() and torch.isfinite(lse).all()
+    assert torch.count_nonzero(out) == 0
