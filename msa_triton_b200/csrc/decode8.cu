@@ -23,11 +23,14 @@
 // that of float32 arithmetic, for 61.3 instead of 62.5 us at 64 requests, 393 instead of 401 us at 256 long ones.)
 // Accumulators, maxima and sums are float32.
 //
-// The values' scales vary by page, so the weights 2^(x_j) vs_j have a running maximum of their own (M' over
-// x_j + log2 vs_j) beside the softmax's M: no weight leaves fp16's range whatever the scales are. What they lose at
-// its lower end, 2^-25, is lost against a largest weight that stands at 2^14 of fp16's 2^16 (the output is scaled back
-// by 2^-14): at most 2^-39 of the row's largest weight times value scale. Weights up to 1 would lose 2^-25 of it, and
-// the sum of many keys far below the largest with them.
+// The values' scales vary by page, so the weights 2^(x_j) vs_j have a reference of their own beside the softmax's M.
+// With vs_j = 2^e_j m_j, 1 <= m_j < 2, they are 2^(x_j - M + e_j - M') m_j, M' an integer near the maximum of
+// x_j - M + e_j: everything in the exponent but x_j - M is exact, however large the logits and far apart the scales (a
+// logarithm of vs_j added to a logit of 1000 would keep 2^-15). Neither M nor M' has to be the maximum itself: they
+// move, with the shuffles and the scaling that takes, only once a key lies more than kSlack above one of them.
+// Weights enter the products 2^kLift higher (taken off the output again): below 2^(kLift + kSlack + 1) < 2^16 in
+// fp16's range, so that what fp16 loses at its lower end, 2^-25, is 2^-38 of the row's largest weight times value scale.
+// Weights up to 1 would lose 2^-25 of it, and the sum of many keys far below the largest with them.
 //
 // A warp works on its own, 32 keys at a time, through a ring of kStages tiles in shared memory that
 // cp.async fills (16 bytes a lane; the 16-byte units of a line are permuted so that neither product's
@@ -46,7 +49,8 @@ constexpr int kWarps = 4;
 constexpr int kTile = 32;      // keys a warp takes at a time
 constexpr int kStages = 2;     // tiles of a warp's ring
 constexpr int kMaxSplits = 8;  // blocks of a cluster
-constexpr int kLift = 14;      // weights relative to the largest times 2^kLift, see below
+constexpr int kLift = 13;      // see above; kLift + kSlack + 1 stays below 16
+constexpr float kSlack = 1.9f;
 
 struct Cache {
   const uint8_t* p;
@@ -70,9 +74,11 @@ struct Params {
   bool uniform;  // 16 keys in a row never leave a page
 };
 
+// (Neither this nor movmatrix is volatile: what they give depends on their operands alone, and in a fixed order
+// they cost registers that spill: 63.5 instead of 61.3 us at 64 requests.)
 __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uint32_t a2, uint32_t a3, uint32_t b0,
                                     uint32_t b1) {
-  asm volatile(
+  asm(
       "mma.sync.aligned.m16n8k16.row.col.f32.f16.f16.f32 {%0, %1, %2, %3}, {%4, %5, %6, %7}, {%8, %9}, "
       "{%0, %1, %2, %3};"
       : "+f"(d[0]), "+f"(d[1]), "+f"(d[2]), "+f"(d[3])
@@ -82,7 +88,7 @@ __device__ __forceinline__ void mma(float (&d)[4], uint32_t a0, uint32_t a1, uin
 // The transposed 8 x 8 matrix of 16-bit elements, row lane / 4, columns 2 (lane % 4) and the next.
 __device__ __forceinline__ uint32_t transpose8(uint32_t x) {
   uint32_t y;
-  asm volatile("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
+  asm("movmatrix.sync.aligned.m8n8.trans.b16 %0, %1;" : "=r"(y) : "r"(x));
   return y;
 }
 
@@ -203,16 +209,10 @@ __device__ __forceinline__ void store_out(void* out, int64_t row, int d, int dim
     }
 }
 
-// 2^x and log2 x by the special function unit (2 ulp; a subnormal result, a weight 2^-126 of the largest, is
-// zero).
+// 2^x by the special function unit (2 ulp; a subnormal result, a weight 2^-126 of the largest, is zero).
 __device__ __forceinline__ float fast_exp2(float x) {
   float y;
   asm("ex2.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
-  return y;
-}
-__device__ __forceinline__ float fast_log2(float x) {
-  float y;
-  asm("lg2.approx.f32 %0, %1;" : "=f"(y) : "f"(x));
   return y;
 }
 
@@ -242,11 +242,12 @@ __device__ __forceinline__ void cluster_arrive() {
 }
 __device__ __forceinline__ void cluster_wait() { asm volatile("barrier.cluster.wait.acquire.aligned;" ::: "memory"); }
 
-// Bytes of a warp's shared memory: its ring (keys, values, their scales, the mask of each tile), its list
-// of block ids; the partial result takes the same place at the end.
+// Bytes of a warp's shared memory: its ring (keys, values, four floats a key: its scale, the value's, and that one's
+// exponent and mantissa once they are split; the mask of each tile), its list of block ids; the partial result takes
+// the same place at the end.
 template <int DP, int HR>
 struct Layout {
-  static constexpr int kStage = 2 * kTile * DP + 2 * kTile * 4 + 16;
+  static constexpr int kStage = 2 * kTile * DP + kTile * 16 + 16;
   static constexpr int kRing = kStages * kStage + 32 * 4;
   static constexpr int kRows = 8 * HR;
   static constexpr int kPitch = DP + 4;  // floats; with part_at, no bank twice when a warp stores its rows
@@ -416,10 +417,10 @@ decode8_kernel(const __grid_constant__ Params p) {
           }
         }
         const int64_t at = here ? (int64_t)page * p.groups + g : 0;
-        cp_async4(base + 2 * kTile * DP + 4 * lane, p.k.scale + at, here);
-        cp_async4(base + 2 * kTile * DP + 4 * (kTile + lane), p.v.scale + at, here);
+        cp_async4(base + 2 * kTile * DP + 16 * lane, p.k.scale + at, here);
+        cp_async4(base + 2 * kTile * DP + 16 * lane + 4, p.v.scale + at, here);
       }
-      if (lane == 0) *reinterpret_cast<uint32_t*>(mine + stage * L::kStage + 2 * kTile * DP + 8 * kTile) = seen;
+      if (lane == 0) *reinterpret_cast<uint32_t*>(mine + stage * L::kStage + 2 * kTile * DP + 16 * kTile) = seen;
       cp_async_commit();
     };
 
@@ -436,12 +437,17 @@ decode8_kernel(const __grid_constant__ Params p) {
       __syncwarp();
       const uint32_t base_k = ring + stage * L::kStage, base_v2 = base_k + kTile * DP;
       float* scales = reinterpret_cast<float*>(mine + stage * L::kStage + 2 * kTile * DP);
-      const uint32_t now = *reinterpret_cast<const uint32_t*>(scales + 2 * kTile);
+      const uint32_t now = *reinterpret_cast<const uint32_t*>(scales + 4 * kTile);
       if (now == 0) {  // no key of this tile is attended (behind the newest token)
         __syncwarp();
         continue;
       }
-      scales[kTile + lane] = fast_log2(scales[kTile + lane]);
+      {  // the value scale as 2^e m, m times 2^kLift; zero and subnormal ones have e = -126
+        const float s = scales[4 * lane + 1];
+        const int e = min(max((int)(__float_as_uint(s) >> 23 & 255), 1), 254);
+        *reinterpret_cast<float2*>(scales + 4 * lane + 2) = make_float2(
+            (float)(e - 127), s * __uint_as_float(max((254u - e) << 23, 0x400000u)) * (1 << kLift));
+      }
       __syncwarp();
       // ---- S^T: x[kt][r][2 a + e] is key 16 kt + n + 8 a, head 8 r + 2 j + e
       float x[kKT][HR][4];
@@ -474,18 +480,23 @@ decode8_kernel(const __grid_constant__ Params p) {
         }
       }
       // ---- softmax weights
-      float top[HR][2], top_v[HR][2], shift[kKT][2];
+      float top[HR][2], top_v[HR][2], base[HR][2], shift[kKT][2], mantissa[kKT][2];
 #pragma unroll
       for (int r = 0; r < HR; ++r)
 #pragma unroll
-        for (int e = 0; e < 2; ++e) top[r][e] = top_v[r][e] = -INFINITY;
+        for (int e = 0; e < 2; ++e) {
+          top[r][e] = top_v[r][e] = -INFINITY;
+          base[r][e] = m_soft[r][e] == -INFINITY ? 0.f : m_soft[r][e];
+        }
 #pragma unroll
       for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
         for (int a = 0; a < 2; ++a) {
           const int key = 16 * kt + n + 8 * a;
-          const float f = scales[key];
-          shift[kt][a] = scales[kTile + key];
+          const float4 of = *reinterpret_cast<const float4*>(scales + 4 * key);
+          const float f = of.x;
+          shift[kt][a] = of.z;
+          mantissa[kt][a] = of.w;
 #pragma unroll
           for (int r = 0; r < HR; ++r)
 #pragma unroll
@@ -501,53 +512,58 @@ decode8_kernel(const __grid_constant__ Params p) {
               for (int r = 0; r < HR; ++r) x[kt][r][2 * a] = x[kt][r][2 * a + 1] = -INFINITY;
             }
       }
-#pragma unroll
-      for (int kt = 0; kt < kKT; ++kt)
-#pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int r = 0; r < HR; ++r)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              top[r][e] = fmaxf(top[r][e], x[kt][r][2 * a + e]);
-              top_v[r][e] = fmaxf(top_v[r][e], x[kt][r][2 * a + e] + shift[kt][a]);
-            }
-      float base[HR][2], base_v[HR][2], alpha[HR][2];
-      bool rescale = false;
+      bool grown = false;
 #pragma unroll
       for (int r = 0; r < HR; ++r)
 #pragma unroll
         for (int e = 0; e < 2; ++e) {
-          const float ms = fmaxf(m_soft[r][e], column_max(top[r][e]));
-          const float mv = fmaxf(m_val[r][e], column_max(top_v[r][e]));
-          base[r][e] = ms == -INFINITY ? 0.f : ms;
-          base_v[r][e] = mv == -INFINITY ? 0.f : mv;
-          l[r][e] *= fast_exp2(m_soft[r][e] - base[r][e]);
-          alpha[r][e] = fast_exp2(m_val[r][e] - base_v[r][e]);
-          rescale = rescale || mv != m_val[r][e];
-          m_soft[r][e] = ms;
-          m_val[r][e] = mv;
-        }
 #pragma unroll
-      for (int kt = 0; kt < kKT; ++kt)
+          for (int kt = 0; kt < kKT; ++kt)
 #pragma unroll
-        for (int a = 0; a < 2; ++a)
-#pragma unroll
-          for (int r = 0; r < HR; ++r)
-#pragma unroll
-            for (int e = 0; e < 2; ++e) {
-              float& y = x[kt][r][2 * a + e];
-              l[r][e] += fast_exp2(y - base[r][e]);
-              y = fast_exp2(y + shift[kt][a] - base_v[r][e]) * (1 << kLift);  // not in the exponent: logits may be large
+            for (int a = 0; a < 2; ++a) {
+              const float y = x[kt][r][2 * a + e];
+              top[r][e] = fmaxf(top[r][e], y);
+              top_v[r][e] = fmaxf(top_v[r][e], y - base[r][e] + shift[kt][a]);
             }
-      if (__any_sync(0xffffffffu, rescale)) {
+          grown = grown || top[r][e] > m_soft[r][e] + kSlack || top_v[r][e] > m_val[r][e] + kSlack;
+        }
+      if (__any_sync(0xffffffffu, grown)) {
 #pragma unroll
         for (int r = 0; r < HR; ++r)
 #pragma unroll
-          for (int t = 0; t < kTiles; ++t)
+          for (int e = 0; e < 2; ++e) {
+            const float ms = fmaxf(m_soft[r][e], column_max(top[r][e]));
+            base[r][e] = ms == -INFINITY ? 0.f : ms;
+            const float delta = m_soft[r][e] - base[r][e];
+            m_soft[r][e] = ms;
+            l[r][e] *= fast_exp2(delta);
+            float tv = -INFINITY;
 #pragma unroll
-            for (int i = 0; i < 4; ++i) o[r][t][i] *= alpha[r][i & 1];
+            for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+              for (int a = 0; a < 2; ++a) tv = fmaxf(tv, x[kt][r][2 * a + e] - base[r][e] + shift[kt][a]);
+            // m_val is relative to m_soft
+            const float before = m_val[r][e] + delta, mv = floorf(fmaxf(before, column_max(tv)));
+            const float alpha = fast_exp2(before - (mv == -INFINITY ? 0.f : mv));
+            m_val[r][e] = mv;
+#pragma unroll
+            for (int t = 0; t < kTiles; ++t) o[r][t][e] *= alpha, o[r][t][2 + e] *= alpha;
+          }
       }
+#pragma unroll
+      for (int r = 0; r < HR; ++r)
+#pragma unroll
+        for (int e = 0; e < 2; ++e) {
+          const float base_v = m_val[r][e] == -INFINITY ? 0.f : m_val[r][e];
+#pragma unroll
+          for (int kt = 0; kt < kKT; ++kt)
+#pragma unroll
+            for (int a = 0; a < 2; ++a) {
+              const float y = x[kt][r][2 * a + e] - base[r][e];
+              l[r][e] += fast_exp2(y);
+              x[kt][r][2 * a + e] = fast_exp2(y + (shift[kt][a] - base_v)) * mantissa[kt][a];
+            }
+        }
       // ---- O^T += V^T P^T
 #pragma unroll
       for (int s = 0; s < kKT; ++s) {
@@ -631,12 +647,12 @@ decode8_kernel(const __grid_constant__ Params p) {
     }
   __syncthreads();
 
+  // m: the softmax's reference; mv: the values', relative to it
   auto finish = [&](int row, int i, float m, float mv, float sum, float4 acc) {
     // no key: zero and -inf; a NaN sum stays one
     const bool none = m == -INFINITY && sum == 0.f;
     // the sum and 2^kLift first: the product stays near the codes, whatever the scales are
-    // (no value scale above zero: mv is -inf, f 0, and a NaN sum or value stays one)
-    const float f = mv == -INFINITY ? 0.f : exp2f(mv - (m == -INFINITY ? 0.f : m)), g = 1.f / (1 << kLift) / sum;
+    const float f = exp2f(mv), g = 1.f / (1 << kLift) / sum;
     store_out<VEC>(p.out, q_row + row, 4 * i, p.dim, p.dtype,
                    none ? make_float4(0.f, 0.f, 0.f, 0.f)
                         : make_float4(acc.x * g * f, acc.y * g * f, acc.z * g * f, acc.w * g * f));
@@ -660,13 +676,18 @@ decode8_kernel(const __grid_constant__ Params p) {
       const float* stats = reinterpret_cast<const float*>(smem + w * L::kBytes) + L::kStats + row;
       ms[w] = stats[0], mvs[w] = stats[kRows];
       m = fmaxf(m, ms[w]);
+    }
+    const float m0 = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int w = 0; w < kWarps; ++w) {
+      mvs[w] += ms[w] - m0;  // relative to the common maximum
       mv = fmaxf(mv, mvs[w]);
     }
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int w = 0; w < kWarps; ++w) {
       const float* from = reinterpret_cast<const float*>(smem + w * L::kBytes);
-      sum += from[L::kStats + 2 * kRows + row] * fast_exp2(ms[w] - (m == -INFINITY ? 0.f : m));
+      sum += from[L::kStats + 2 * kRows + row] * fast_exp2(ms[w] - m0);
       add(acc, *reinterpret_cast<const float4*>(from + part_at<DP, HR>(row, i)),
           fast_exp2(mvs[w] - (mv == -INFINITY ? 0.f : mv)));
     }
@@ -696,9 +717,14 @@ decode8_kernel(const __grid_constant__ Params p) {
       s[r] = stats[from * kRows + row];
       part[r] = shares[from * share + k];
       m = fmaxf(m, s[r].x);
+    }
+    const float m0 = m == -INFINITY ? 0.f : m;
+#pragma unroll
+    for (int r = 0; r < kMaxSplits; ++r) {
+      s[r].y += s[r].x - m0;
       mv = fmaxf(mv, s[r].y);
     }
-    const float m0 = m == -INFINITY ? 0.f : m, mv0 = mv == -INFINITY ? 0.f : mv;
+    const float mv0 = mv == -INFINITY ? 0.f : mv;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
 #pragma unroll
     for (int r = 0; r < kMaxSplits; ++r)

@@ -93,3 +93,28 @@ def test_no_value_scale_left_far_below_zero(dtype, cuda_device):
     out, lse = run(made, 128, cuda_device)
     assert (lse < -100).any() and torch.isfinite(lse).all()
     assert torch.count_nonzero(out) == 0
+
+
+@pytest.mark.parametrize("scale", [1.3 * 2.0 ** -6, 1.7 * 2.0 ** -100, 1.1 * 2.0 ** 60, 2.0 ** 118])
+@pytest.mark.parametrize("size", [0.1, 60.0, 1e4, 1e7])
+def test_equal_logits_average_the_values(size, scale, cuda_device):
+    """One key to a request, or several with the same codes: whatever the logits and the value scales are, the weights
+    are equal, and the output is the mean of the values: 2^-21 for the weights' two terms and the powers of two, u a key
+    and 64 of the values' sizes."""
+    made = make_case([1, 1, 2, 70, 130], 2, 8, 64, 128, 16, 2, torch.float32, seed=5)
+    q, k, v, ks, vs, table, lens, ids = made
+    k.copy_(torch.randn(1, 1, 2, 64, generator=torch.Generator().manual_seed(3)).to(FP8).expand(k.shape))
+    ks.fill_(float(ks[0, 0]))
+    gen = torch.Generator().manual_seed(1)
+    vs.copy_(scale * (1 + torch.rand(vs.shape, generator=gen)))
+    q.mul_(size)
+    out, _ = run(made, 128, cuda_device)
+    out = out.cpu().double()
+    for b, n in enumerate(lens.tolist()):
+        at = torch.arange(n)
+        page = table[b, at // 16].long()
+        x = v[page, at % 16].float().double() * vs[page].double()[..., None]
+        want, sizes = (y.mean(0).repeat_interleave(8, 0) for y in (x, x.abs()))
+        off = (out[b] - want).abs()
+        bound = (2.0 ** -21 + (n + 64) * R.U) * sizes + R.U * want.abs()
+        assert float((off - bound).max()) <= 0, f"{n} keys: {float((off / bound.clamp(min=1e-300)).max())} of the bound"
