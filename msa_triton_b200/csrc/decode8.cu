@@ -290,7 +290,7 @@ decode8_kernel(const __grid_constant__ Params p) {
   int id = lane < p.topk ? ids[lane] : -1;
   const int pos = p.seq_lens[b] - 1;
   const int64_t q_row = (int64_t)b * p.q_heads + (int64_t)g * h_all + h0;
-  // ---- queries: fragments of q / 2^e, and the factor 2^e * scale * log2(e) of each row
+  // ---- queries: fragments of q / 2^e, and the factor 2^e of each row
   // (read after the first copies are on their way)
   uint32_t qa[HR][kSteps][2] = {}, qb[SPLIT ? HR : 1][SPLIT ? kSteps : 1][2] = {};
   float qf[HR][2] = {};  // of the heads 8 r + 2 j + e, the columns of this lane
@@ -307,11 +307,10 @@ decode8_kernel(const __grid_constant__ Params p) {
       }
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 1));
       top = fmaxf(top, __shfl_xor_sync(0xffffffffu, top, 2));
-      // 2^e with top < 2^(e+1); nothing is scaled in an all-zero, subnormal or infinite row
-      const uint32_t e = __float_as_uint(top) >> 23;
-      const bool scaled = e >= 2 && e <= 252;
-      const float inv = scaled ? __uint_as_float((254 - e) << 23) : 1.f;
-      const float f = p.scale_log2 * (scaled ? __uint_as_float(e << 23) : 1.f);
+      // 2^e with top < 2^(e+1), or < 2^(e+2) at the range's upper end; subnormal rows come out below 1, with all the
+      // bits that they have
+      const uint32_t e = min(max(__float_as_uint(top) >> 23, 1u), 253u);
+      const float inv = __uint_as_float((254 - e) << 23), f = __uint_as_float(e << 23);
       qf[r][0] = __shfl_sync(0xffffffffu, f, 8 * j);
       qf[r][1] = __shfl_sync(0xffffffffu, f, 8 * j + 4);
 #pragma unroll
@@ -442,11 +441,13 @@ decode8_kernel(const __grid_constant__ Params p) {
         __syncwarp();
         continue;
       }
-      {  // the value scale as 2^e m, m times 2^kLift; zero and subnormal ones have e = -126
+      {  // the key scale times scale * log2(e); the value scale as 2^e m, m times 2^kLift (zero and subnormal ones have
+         // e = -126)
         const float s = scales[4 * lane + 1];
         const int e = min(max((int)(__float_as_uint(s) >> 23 & 255), 1), 254);
-        *reinterpret_cast<float2*>(scales + 4 * lane + 2) = make_float2(
-            (float)(e - 127), s * __uint_as_float(max((254u - e) << 23, 0x400000u)) * (1 << kLift));
+        *reinterpret_cast<float4*>(scales + 4 * lane) =
+            make_float4(scales[4 * lane] * p.scale_log2, s, (float)(e - 127),
+                        s * __uint_as_float(max((254u - e) << 23, 0x400000u)) * (1 << kLift));
       }
       __syncwarp();
       // ---- S^T: x[kt][r][2 a + e] is key 16 kt + n + 8 a, head 8 r + 2 j + e

@@ -118,3 +118,38 @@ def test_equal_logits_average_the_values(size, scale, cuda_device):
         off = (out[b] - want).abs()
         bound = (2.0 ** -21 + (n + 64) * R.U) * sizes + R.U * want.abs()
         assert float((off - bound).max()) <= 0, f"{n} keys: {float((off / bound.clamp(min=1e-300)).max())} of the bound"
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("power", [-133, -126, -118, 125, 126, 127])
+def test_queries_at_the_ends_of_the_range(power, dtype, cuda_device):
+    """Queries around 2^power with key scales and a factor that bring their logits back to ordinary size."""
+    made = make_case([90, 200], 2, 8, 64, 128, 16, 2, dtype, seed=17)
+    q, k, v, ks, vs, *_ = made
+    signs = torch.randn(q.shape, generator=torch.Generator().manual_seed(4))
+    q.copy_((signs.sign() * (1 + signs.abs().clamp(max=0.9))).double().mul(2.0 ** power).to(dtype))
+    scale = 2.0 ** -20 if power > 0 else 2.0 ** 20
+    ks.copy_((ks.double() * (2.0 ** -power / scale / 8)).float())
+    assert torch.isfinite(q.float()).all() and (ks >= torch.finfo(torch.float32).tiny).all() and torch.isfinite(ks).all()
+    check(made, 128, run(made, 128, cuda_device, scale=scale), CUT, scale=scale)
+
+
+def test_logits_across_the_range(cuda_device):
+    """Logits near both ends of float32: one key outweighs whatever came before it."""
+    made = make_case([256], 1, 4, 64, 32, 32, 8, torch.float32, seed=18)
+    q, k, v, ks, vs, table, lens, ids = made
+    q.zero_()
+    q[..., 0] = 1.0
+    k.zero_()
+    for i in range(8):
+        k[int(table[0, i]), :, 0, 0] = torch.tensor(-448.0 if i < 4 else 448.0).to(FP8)
+    k[int(table[0, 6]), 5:, 0, 0] = 0
+    ks.fill_(2.0 ** 119)
+    ids.copy_(torch.arange(8, dtype=torch.int32))
+    out, lse = run(made, 32, cuda_device, scale=0.5)
+    keys = torch.tensor([i * 32 + j for i in range(4, 8) for j in range(32) if i != 6 or j < 5])
+    page = table[0][keys // 32].long()
+    x = v[page, keys % 32, 0].float().double() * vs[page, 0].double()[:, None]
+    off = (out[0].cpu().double() - x.mean(0)).abs()
+    assert float((off - (2.0 ** -21 + (len(keys) + 64) * R.U) * x.abs().mean(0)).max()) <= 0
+    assert torch.isfinite(lse).all()
