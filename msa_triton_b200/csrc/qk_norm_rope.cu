@@ -398,7 +398,11 @@ __global__ void __launch_bounds__(kWarps * 32) any_kernel(const __grid_constant_
     const T* g = BWD ? static_cast<const T*>(s.g) + t * s.g_ts + h * s.g_hs : nullptr;
     const int64_t pos = positions.of(p, t);
     const bool inside = pos >= 0 && pos < p.table_rows;
+    // a position outside the table turns nothing (the row is NaN through r): the table may have no rows at all
     const float* angles = p.table + (inside ? pos : 0) * p.rotary;
+    auto turn = [&](float& a, float& b, int unit, float sign) {
+      if (inside) rotate_pair(a, b, angles[unit], sign * angles[p.rotary / 2 + unit]);
+    };
     float v[NU][2], u[BWD ? NU : 1][2], ss = 0.f, dot = 0.f;
 #pragma unroll
     for (int j = 0; j < NU; ++j) {
@@ -415,7 +419,7 @@ __global__ void __launch_bounds__(kWarps * 32) any_kernel(const __grid_constant_
         u[j][0] = to_float(g[e.a]);
         if (e.b >= 0) {
           u[j][1] = to_float(g[e.b]);
-          rotate_pair(u[j][0], u[j][1], angles[unit], -angles[p.rotary / 2 + unit]);
+          turn(u[j][0], u[j][1], unit, -1.f);
         }
         dot = fmaf(u[j][0] * load_weight(s.w, e.a, p.w_dtype), v[j][0], dot);
         if (e.b >= 0) dot = fmaf(u[j][1] * load_weight(s.w, e.b, p.w_dtype), v[j][1], dot);
@@ -441,7 +445,7 @@ __global__ void __launch_bounds__(kWarps * 32) any_kernel(const __grid_constant_
       } else {
         ya = v[j][0] * r * wa;
         yb = v[j][1] * r * wb;
-        if (e.b >= 0) rotate_pair(ya, yb, angles[unit], angles[p.rotary / 2 + unit]);
+        if (e.b >= 0) turn(ya, yb, unit, 1.f);
       }
       if (out) {
         out[e.a] = from_float<T>(ya);
