@@ -564,8 +564,8 @@ extern "C" int msa_cache_append(const void* k, const void* v, int dtype, int64_t
                 "msa_cache_append: bad sizes");
   MSA_CHECK_ARG(cu_seqlens || total_tokens == batch, "msa_cache_append: without cu_seqlens one token per request");
   MSA_CHECK_ARG(rotary_dim >= 0 && rotary_dim % 2 == 0 && rotary_dim <= head_dim && table_rows >= 0 &&
-                    (rotary_dim == 0 || rope_table),
-                "msa_cache_append: rotary_dim must be even and at most head_dim");
+                    (rotary_dim == 0 || table_rows == 0 || rope_table),  // an empty table has no address
+                "msa_cache_append: rotary_dim must be even and at most head_dim, and needs a table");
   // nothing to store; empty tensors have no address
   if (batch == 0 || total_tokens == 0 || max_pages == 0 || num_pages == 0) return MSA_OK;
   MSA_CHECK_ARG(k && k_cache && block_table && seq_lens && !v == !v_cache,
