@@ -8,6 +8,9 @@ stores the newest tokens of every request, rotating the keys on the way:
     m3_cache_append(k, v, k_cache, v_cache, block_table, seq_lens, cu_seqlens=cu)         # packed chunks
     m3_cache_append(index_k, None, index_k_cache, None, block_table, seq_lens)            # the indexer's keys
 
+(``m3_index_score_decode`` reads the indexer's cache in the type of its queries only: keep that one in 16 or
+32 bits.)
+
 8-bit caches are ``torch.float8_e4m3fn`` with float32 scales ``[P, G]``, one per page and
 head: a code ``c`` stands for ``c * scale``. The append chooses powers of two, the smallest
 with every value at most ``448 * scale`` (e4m3 is a floating format, so that costs no

@@ -272,13 +272,16 @@ __device__ __forceinline__ float block_amax(float v, float* red) {
 }
 
 // Chunks: a block takes HC heads (4, or 1 of a tensor with fewer) of a (request, page), of k or v. It reads the rows
-// twice, once for the heads' maxima and once for the codes: the second time they come from L2 (a wave of blocks
-// holds some 50 MB, half the L2). That keeps whole kilobytes of a token's heads together and one set of angles for
-// them, and holds nothing on the way. The maximum takes whatever is there: NaN drops out of fmaxf by itself, and
-// only a page that holds an infinity is looked through again for its finite values.
+// twice, once for the heads' maxima and once for the codes. That keeps whole kilobytes of a token's heads together and
+// one set of angles for them, and holds nothing on the way. The second time the rows come from L2 as long as those of
+// the blocks that run together fit it: four blocks an SM of 128 rows of 4 heads of 128 16-bit elements, 78 of its
+// 126 MB. The maximum takes whatever is there: NaN drops out of fmaxf by itself, and only a page that holds an
+// infinity is looked through again for its finite values.
 // Measured: 32768 tokens, 8 heads of 128 (bf16), pages of 128: 60 us, 3.5 TB/s of the 210 MB that must move, 54% of
 // the copy rate; DRAM reads are 1.1 times the input, so the second pass does hit L2. Issue slots are 66% busy:
-// what is left is instructions (138 a lane for the two passes over a 16-byte piece). A head at a time to a
+// what is left is instructions (138 a lane for the two passes over a 16-byte piece). Where the blocks' rows outgrow L2,
+// DRAM is read twice: float32 inputs (155 MB) 1.6 times the input, 90 us of a floor of 53; pages of 512 (264
+// blocks, 138 MB) 1.8 times, 86 us of 32; both 2.0 times, 107 us of 53. A head at a time to a
 // block, its rows held in registers or copied ahead into shared memory, took 75-93 us (256-byte pieces two
 // kilobytes apart); eight heads 87 us (too few blocks).
 template <typename T, int LPR, bool INTER, int HC>

@@ -760,10 +760,10 @@ int launch(Params p, int batch, cudaStream_t st) {
   // least in merging, but the blocks behind the last whole wave would run on a chip that is mostly idle. If they are
   // no more than half a wave, as many items, or a sixth of a wave if that is more, go to pairs of blocks, first: the
   // lone blocks behind them start at another time than the others, and the pairs' slots take the last ones. Measured
-  // (16 blocks, 8 groups of 128; a wave is 444 items): 64 requests 57.9 us (77.1 with lone blocks alone, 67 with
-  // clusters of 4, 58.4 with pairs for the 68 items over and above the wave alone), 56 requests 55.3 (60.3, 69,
-  // 56.8), 128 requests 103 (114.5, 116, 103); 80 requests, 196 items behind the wave, 73 (79.8); 96, 324 items
-  // behind it: 81.6 alone, 89 with pairs.
+  // (16 blocks, 8 groups of 128; a wave is 444 items): 64 requests 61.7 us (70.4 with lone blocks alone, 69.6 with
+  // clusters of 4, 62.1 with pairs for the 68 items over and above the wave alone), 56 requests 56.6 (57.6, 69.5,
+  // 57.3), 128 requests 103.3 (110, 114, 103.8); 80 requests, 196 items behind the wave, 71.6 (80.7); 96, 324 items
+  // behind it: 83.4 alone, 90.4 with pairs.
   const int64_t head_tiles = ceil_div(p.q_heads / p.groups, 16), items = (int64_t)batch * p.groups;
   const int64_t slots = std::max<int64_t>(148 * per_sm / head_tiles, 1), behind = items % slots;
   const int64_t tiles = (int64_t)p.topk * ((p.block + kTile - 1) / kTile);

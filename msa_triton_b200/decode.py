@@ -113,7 +113,10 @@ def m3_sparse_decode(q, k_cache, v_cache, block_table, seq_lens, indices, *, blo
 
     With 8-bit caches (``torch.float8_e4m3fn``), ``k_scale`` / ``v_scale`` (float32 ``[P,G]``) hold
     what ``m3_cache_append`` keeps: a code of page p and head g stands for ``code * scale[p, g]``.
-    The caches may then have any strides with dense head rows."""
+    The caches may then have any strides with dense head rows, and D is at most 256. Codes enter the
+    products exactly, 16-bit queries but for elements 2^-14 below their head's largest (kept to 2^-25 of it);
+    a softmax weight times its value scale keeps 2^-22 of itself, or 2^-38 of its row's largest one where
+    that is more. Sums are float32, and the output is rounded once, for every type."""
     if q.ndim != 3 or k_cache.ndim != 4 or v_cache.shape != k_cache.shape:
         raise ValueError("expected q[B,Hq,D] and k_cache/v_cache[P,S,G,D]")
     batch, hq, dim = q.shape
